@@ -164,6 +164,17 @@ _SIGNATURES = {
     "tq_lightning_chunked": [_c_ptr, _c_i64, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_i64, _c_int, _c_int, _c_int, _c_int, _c_int,
                              _c_ptr, _c_int, _c_ptr, _c_ptr],
     "tq_lightning_out": [_c_ptr, _c_ptr, _c_i64, _c_ptr, _c_int, _c_f32, _c_ptr, _c_int, _c_int, _c_ptr],
+    "tq_e4m3_write": [_c_ptr, _c_i64, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_int, _c_int, _c_f32, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int,
+                      _c_int, _c_int, _c_int, _c_int, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_int,
+                      _c_int, _c_ptr],
+    "tq_e4m3_choose": [_c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int,
+                       _c_ptr],
+    "tq_e4m3_move": [_c_ptr, _c_ptr, _c_int, _c_ptr, _c_int, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int,
+                     _c_int, _c_int, _c_ptr],
+    "tq_e4m3_attention_scratch": [_c_int] * 7,
+    "tq_e4m3_attention": [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_f32, _c_f32, _c_ptr,
+                          _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_ptr,
+                          _c_int, _c_int, _c_int, _c_ptr],
 }
 # entry points that only one of the two libraries has
 _OPTIONAL = {
@@ -248,6 +259,7 @@ def library(dtype) -> ctypes.CDLL:
     lib.tq_sample_topp_scratch.restype = _c_i64
     lib.tq_delta_state_floats.restype = _c_i64
     lib.tq_delta_chunk_scratch.restype = _c_i64
+    lib.tq_e4m3_attention_scratch.restype = _c_i64
     for fn in ("tq_attention_decode_scratch", "tq_attention_f32_scratch"):
         if hasattr(lib, fn):
             getattr(lib, fn).restype = _c_i64
@@ -301,7 +313,8 @@ _KIND = {"gemm": "matmul", "gemm_mfma": "matmul", "gemm_f32": "matmul", "gemm_pa
          "mm_scan": "attn", "mm_chunked": "attn", "mm_out": "attn", "mm_decode": "attn",
          "lightning_scan": "attn", "lightning_chunked": "attn", "lightning_out": "attn",
          "ssd_prep": "attn", "ssd_scan": "attn", "ssd_chunked": "attn", "ssd_decode": "attn", "ssd_out": "attn",
-         "row_norm_kv_write": "attn", "diff_prep_kv_write": "attn", "diff_combine": "attn"}
+         "row_norm_kv_write": "attn", "diff_prep_kv_write": "attn", "diff_combine": "attn",
+         "rope_kv_write_e4m3": "attn", "attention_e4m3": "attn", "evict_choose": "attn", "evict_move": "attn"}
 
 
 def profile_begin() -> None:
@@ -1329,6 +1342,211 @@ def attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, lay
 def attention_writes_into(act, head_dim: int, scale: float) -> bool:
     """Whether ``attention`` takes ``out``: heads and scale that the bfloat16 matrix-core kernels run (with pages of whole tiles)."""
     return dtype_name(act) == "bfloat16" and head_dim % 16 == 0 and head_dim <= 512 and scale > 0
+
+
+# ------------------------------------------------------------------ a cache in 8 bits
+E4M3_BLOCK = 16      # positions that share a scale
+
+
+@dataclasses.dataclass
+class E4m3Pages:
+    """Pages of keys and values as e4m3 codes with a scale, a power of two, for each block of 16 positions of a layer's kv head.
+
+    ``k``, ``v`` float8_e4m3fn [pages, layers, kv heads, page_size * head_dim]; ``k_scale``, ``v_scale`` float32 [pages, layers, kv
+    heads, page_size / 16]; ``weight`` (None: not kept) float32 [pages, layers, kv heads, page_size], the attention weight that each
+    position has received; ``table`` int32 [slots, logical pages], -1 where there is none.  page_size is a multiple of 64, head_dim a
+    multiple of 16 up to 256.  A number is its code times its block's scale.  Within a tile of 64 positions keys lie [head_dim / 16]
+    [64 positions][16 numbers] and values [head_dim][4][4][4], position 16 j + 4 c + i at [c][j][i].
+
+    The scale is the smallest power of two, 2^-100 at least, whose 448 fold is no smaller than the block's largest magnitude: a
+    number of the block is off by at most 2^-4 of itself, or 2^-10 of the scale where that is more.  A block that a later token makes
+    larger takes the larger scale, and what it holds is rounded to that (exact down to 2^-6 of the scale).  A token
+    whose key or value of a head holds a number that is not finite (or is 2^120 or more) keeps NaN for its key: every output that sees
+    it is NaN, no other is touched."""
+    k: torch.Tensor
+    v: torch.Tensor
+    k_scale: torch.Tensor
+    v_scale: torch.Tensor
+    table: torch.Tensor
+    weight: torch.Tensor | None = None
+
+    @classmethod
+    def empty(cls, n_pages: int, layers: int, num_kv_heads: int, head_dim: int, page_size: int, table: torch.Tensor,
+              weights: bool = False) -> "E4m3Pages":
+        """Pages that hold nothing yet, on the table's device: zeros, as tiles that a sequence fills in part are read whole (and
+        masked)."""
+        dev, rows = table.device, (n_pages, layers, num_kv_heads)
+        pool = [torch.zeros((*rows, page_size * head_dim), dtype=torch.uint8, device=dev).view(torch.float8_e4m3fn) for _ in range(2)]
+        scale = [torch.zeros((*rows, page_size // E4M3_BLOCK), dtype=torch.float32, device=dev) for _ in range(2)]
+        return cls(*pool, *scale, table, torch.zeros((*rows, page_size), dtype=torch.float32, device=dev) if weights else None)
+
+    @property
+    def page_size(self) -> int:
+        return self.k_scale.shape[-1] * E4M3_BLOCK
+
+    @property
+    def head_dim(self) -> int:
+        return self.k.shape[-1] // self.page_size
+
+    def check(self, k: str, device, layer: int = 0) -> None:
+        for name, t, dtype in (("k", self.k, torch.float8_e4m3fn), ("v", self.v, torch.float8_e4m3fn), ("k_scale", self.k_scale, torch.float32),
+                               ("v_scale", self.v_scale, torch.float32), ("weight", self.weight, torch.float32)):
+            if t is not None:
+                _check(t, k, name, dtype)
+                _need(t.dim() == 4 and t.shape[:3] == self.k.shape[:3] and t.device == device, k,
+                      lambda: f"{name} must be [pages, layers, kv heads, ...] as the other pools are, on the same GPU, is {tuple(t.shape)}")
+        _check(self.table, k, "table", torch.int32)
+        _need(self.table.dim() == 2 and self.table.device == device, k, "table must be [slots, pages] on the same GPU")
+        ps = self.page_size
+        _need(ps > 0 and ps % 64 == 0, k, lambda: f"pages must hold a multiple of 64 positions, hold {ps}")
+        _need(self.k.shape[3] % ps == 0 and self.v.shape == self.k.shape and self.v_scale.shape == self.k_scale.shape, k,
+              "pools of keys and values must have one shape, page_size * head_dim numbers to a page's head")
+        _need(self.head_dim % 16 == 0 and 16 <= self.head_dim <= 256, k,
+              lambda: f"head size {self.head_dim} is none of the multiples of 16 up to 256 that 8-bit pages take")
+        _need(self.weight is None or self.weight.shape[3] == ps, k, "weight must have a number for every position")
+        _need(0 <= layer < self.k.shape[1], k, lambda: f"layer {layer} is none of the pages' {self.k.shape[1]}")
+
+
+def _e4m3_runs(k: str, runs: dict, pages: E4m3Pages, T: int, device) -> int:
+    B = runs["slots"].numel()
+    _check(runs["cu_seqlens"], k, "cu_seqlens", torch.int32, (B + 1,))
+    _check(runs["slots"], k, "slots", torch.int32, (B,))
+    _check(runs["start"], k, "start", torch.int32, (B,))
+    _need(all(runs[n].device == device for n in ("cu_seqlens", "slots", "start")), k, "the runs must lie on the same GPU")
+    _need(0 < int(runs["max_end"]) <= pages.table.shape[1] * pages.page_size, k, "positions reach beyond the page table")
+    _need(1 <= int(runs["max_new"]) <= T and (not runs["decode"] or T == B), k, "decoding brings one token per sequence")
+    return B
+
+
+def _same_device(k: str, device) -> None:
+    _need(device.index == torch.cuda.current_device(), k, lambda: f"the tensors lie on {device}, which is not the current device")
+
+
+def rope_kv_write_e4m3(qkv: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, pairing: int, rotary_dim: int,
+                       pages: E4m3Pages, layer: int, num_heads: int, act, runs: dict, bias: torch.Tensor | None = None,
+                       amplitude: float = 1.0, write: bool = True) -> torch.Tensor:
+    """``rope_kv_write`` into pages of 8 bits: rotates queries and keys, returns the queries [T, nh * hd] and writes keys and values
+    of layer ``layer`` as codes.  ``positions`` [T] are what the rotation turns by (the product of position and frequency is taken
+    exactly, not rounded to 32 bits first); the places in the cache are the runs' (``start`` and on), which differ from them where a
+    sequence has let positions go.  ``runs`` as for ``attention``; no slot may stand in it twice.  The new places' weights
+    start at zero.  ``write`` False: the queries alone, for a layer that reads another layer's cache (``qkv`` then holds no keys
+    and values)."""
+    k = "rope_kv_write_e4m3"
+    T = positions.numel()
+    _check(positions, k, "positions", torch.int32, (T,))
+    pages.check(k, positions.device, layer)
+    _same_device(k, positions.device)
+    nkv, hd = pages.k.shape[2], pages.head_dim
+    width = (num_heads + (2 * nkv if write else 0)) * hd
+    _need(num_heads >= 1 and T >= 1, k, "there must be a head and a token")
+    _need(isinstance(qkv, torch.Tensor) and qkv.device == positions.device and qkv.dtype == torch.float32 and tuple(qkv.shape) == (T, width)
+          and qkv.stride(1) == 1 and (qkv.stride(0) >= width or T == 1), k,
+          lambda: f"qkv must be float32 [{T}, {width}] on the GPU with unit stride along its rows")
+    _need((T == 1 or qkv.stride(0) % 4 == 0) and qkv.data_ptr() % 16 == 0, k, "rows of qkv must start at multiples of 16 bytes")
+    if bias is not None:
+        _check(bias, k, "bias", tuple(_WTYPE), (width,))
+    _check(inv_freq, k, "inv_freq", torch.float32)
+    _need(0 <= rotary_dim <= hd and rotary_dim % 2 == 0 and pairing in (0, 1) and (rotary_dim == 0 or inv_freq.numel() * 2 == rotary_dim), k,
+          lambda: f"inv_freq must hold rotary_dim/2 = {rotary_dim // 2} entries, for at most a head's {hd} numbers")
+    B = _e4m3_runs(k, runs, pages, T, positions.device)
+    q = torch.empty((T, num_heads * hd), dtype=ACT_DTYPES[dtype_name(act)], device=positions.device)
+    ld = qkv.stride(0) if T > 1 else width
+    _run(k, library(act).tq_e4m3_write(
+        _ptr(qkv), ld, _ptr(bias), _WTYPE[bias.dtype] if bias is not None else 0, _ptr(positions), _ptr(inv_freq), pairing, rotary_dim,
+        float(amplitude), _ptr(runs["cu_seqlens"]), _ptr(runs["slots"]), _ptr(runs["start"]), _ptr(q), T, B, int(runs["max_new"]), num_heads,
+        nkv if write else 0, hd, _ptr(pages.k) if write else None, _ptr(pages.v) if write else None, _ptr(pages.k_scale), _ptr(pages.v_scale),
+        _ptr(pages.weight), _ptr(pages.table), pages.table.shape[1], pages.page_size, pages.k.shape[1] * nkv, layer * nkv, _stream()))
+    return q
+
+
+def attention_e4m3(q: torch.Tensor, pages: E4m3Pages, layer: int, num_heads: int, window: int | None, scale: float, act, runs: dict,
+                   softcap: float | None = None, distance_bias: tuple[torch.Tensor, torch.Tensor] | None = None,
+                   chunk: int | None = None, sink: torch.Tensor | None = None, add_weights: bool = False) -> torch.Tensor:
+    """``attention`` over pages of 8 bits: each token attends to its sequence's cached positions up to its own; returns [T, nh * hd].
+    Places count here (the runs'), not the positions that keys were rotated by.  The options are ``attention``'s.  ``add_weights``:
+    every position's number in ``pages.weight`` is raised by the weights it receives from the step's tokens and the heads of its kv head,
+    exp(score) over the softmax's denominator (sums in a fixed order: the same step gives the same bits).  A row whose scores are
+    all -inf is 0 and gives no weight."""
+    k = "attention_e4m3"
+    adt = ACT_DTYPES[dtype_name(act)]
+    _need(isinstance(q, torch.Tensor) and q.is_cuda and q.dim() == 2, k, "q must be [T, heads * head_dim] on the GPU")
+    pages.check(k, q.device, layer)
+    _same_device(k, q.device)
+    T, nkv, hd = q.shape[0], pages.k.shape[2], pages.head_dim
+    _check(q, k, "q", adt, (T, num_heads * hd))
+    _need(q.data_ptr() % 16 == 0, k, "q must start at a multiple of 16 bytes")
+    _need(num_heads >= 1 and num_heads % nkv == 0, k, "heads must be a multiple of kv heads")
+    _need(math.isfinite(scale), k, "scale must be finite")
+    _need((window is None or window >= 1) and (chunk is None or chunk >= 1) and (softcap is None or softcap > 0), k,
+          "window, chunk and softcap must be positive")
+    r1 = r2 = None
+    if distance_bias is not None:
+        r1, r2 = distance_bias
+        _check(r1, k, "r1", torch.float32, (num_heads,))
+        _check(r2, k, "r2", torch.float32, (num_heads,))
+    if sink is not None:
+        _check(sink, k, "sink", torch.float32, (num_heads,))
+    _need(not add_weights or pages.weight is not None, k, "these pages keep no weights")
+    B = _e4m3_runs(k, runs, pages, T, q.device)
+    lib, decode = library(act), int(bool(runs["decode"]))
+    out = torch.empty_like(q)
+    n = lib.tq_e4m3_attention_scratch(T, B, num_heads, hd, int(runs["max_end"]), decode, int(add_weights))
+    scratch = torch.empty((n,), dtype=torch.float32, device=q.device) if n else None
+    _run(k, lib.tq_e4m3_attention(
+        _ptr(q), _ptr(out), _ptr(runs["cu_seqlens"]), _ptr(runs["slots"]), _ptr(runs["start"]), T, B, num_heads, nkv, hd, int(window or 0),
+        float(scale), float(softcap or 0.0), _ptr(r1), _ptr(r2), int(chunk or 0), _ptr(sink), _ptr(pages.k), _ptr(pages.v),
+        _ptr(pages.k_scale), _ptr(pages.v_scale), _ptr(pages.weight) if add_weights else None, _ptr(pages.table), pages.table.shape[1],
+        pages.page_size, pages.k.shape[1] * nkv, layer * nkv, _ptr(scratch), decode, int(runs["max_new"]), int(runs["max_end"]), _stream()))
+    return out
+
+
+def evict_choose(pages: E4m3Pages, slots: torch.Tensor, lengths: torch.Tensor, max_length: int, keep: int, first: int = 0,
+                 recent: int = 0, act="bfloat16") -> torch.Tensor:
+    """The positions that the sequences in ``slots`` [B] keep of the ``lengths`` [B] they hold (int32, at most ``max_length``): for
+    every layer and kv head the first ``first``, the last ``recent`` and, of the others, those with the largest ``pages.weight``, ``keep``
+    in all; of equal weights the lower position stays, and NaN counts as the largest.  int32 [B, layers, kv heads, keep] in ascending
+    order.  A sequence of ``keep`` positions or fewer keeps them all, with -1 behind them."""
+    k = "evict_choose"
+    _need(isinstance(slots, torch.Tensor) and slots.is_cuda and slots.dim() == 1, k, "slots must be [B] on the GPU")
+    B = slots.numel()
+    _check(slots, k, "slots", torch.int32, (B,))
+    _check(lengths, k, "lengths", torch.int32, (B,))
+    pages.check(k, slots.device)
+    _same_device(k, slots.device)
+    _need(lengths.device == slots.device, k, "lengths must lie on the same GPU")
+    _need(pages.weight is not None, k, "these pages keep no weights")
+    _need(keep >= 1 and first >= 0 and recent >= 0 and first + recent <= keep, k,
+          lambda: f"the first {first} and last {recent} positions must lie within the {keep} that stay")
+    _need(0 <= max_length <= pages.table.shape[1] * pages.page_size, k, "positions reach beyond the page table")
+    layers, nkv = pages.k.shape[1:3]
+    kept = torch.empty((B, layers, nkv, keep), dtype=torch.int32, device=slots.device)
+    _run(k, library(act).tq_e4m3_choose(_ptr(slots), _ptr(lengths), B, int(max_length), int(keep), int(first), int(recent), _ptr(kept),
+                                        _ptr(pages.weight), _ptr(pages.table), pages.table.shape[0], pages.table.shape[1],
+                                        pages.page_size, layers * nkv, _stream()))
+    return kept
+
+
+def evict_move(pages: E4m3Pages, src_slots: torch.Tensor, dst_slots: torch.Tensor, kept: torch.Tensor, act="bfloat16") -> None:
+    """Copies the positions ``kept`` [B, layers, kv heads, keep] (as ``evict_choose`` gives them, in ascending order; -1: none) of the
+    sequences in ``src_slots`` to places 0, 1, .. of ``dst_slots``, keys, values and weights.  The slots' pages must be different ones: nothing
+    is copied in place.  A block's scale becomes the largest of its rows'; what lies behind the last row in its page becomes zero.  A
+    row of the table that is -1 where a page is written, or a slot outside the table, is passed over."""
+    k = "evict_move"
+    _need(isinstance(src_slots, torch.Tensor) and src_slots.is_cuda and src_slots.dim() == 1, k, "src_slots must be [B] on the GPU")
+    B = src_slots.numel()
+    _check(src_slots, k, "src_slots", torch.int32, (B,))
+    _check(dst_slots, k, "dst_slots", torch.int32, (B,))
+    pages.check(k, src_slots.device)
+    _same_device(k, src_slots.device)
+    layers, nkv = pages.k.shape[1:3]
+    _check(kept, k, "kept", torch.int32)
+    _need(kept.dim() == 4 and tuple(kept.shape[:3]) == (B, layers, nkv) and kept.shape[3] >= 1, k,
+          lambda: f"kept must be [{B}, {layers}, {nkv}, keep]")
+    _need(dst_slots.device == src_slots.device and kept.device == src_slots.device, k, "dst_slots and kept must lie on the same GPU")
+    _need(kept.shape[3] <= pages.table.shape[1] * pages.page_size, k, "positions reach beyond the page table")
+    _run(k, library(act).tq_e4m3_move(_ptr(src_slots), _ptr(dst_slots), B, _ptr(kept), kept.shape[3], pages.head_dim, _ptr(pages.k),
+                                      _ptr(pages.v), _ptr(pages.k_scale), _ptr(pages.v_scale), _ptr(pages.weight), _ptr(pages.table),
+                                      pages.table.shape[0], pages.table.shape[1], pages.page_size, layers * nkv, _stream()))
 
 
 # ------------------------------------------------------------------ routing
