@@ -42,7 +42,7 @@ struct E4m3Attn {
   int max_runs;
   float* scores;                // decoding with weights: [B][nh][ld_scores], a column's scores in units of log2
   int64_t ld_scores;
-  float* lse;                   // with weights: [T][nh] log2 of a row's sum of 2^score, the sink's included
+  float* lse;                   // prompts with weights: [T][nh] log2 of a row's sum of 2^score, the sink's included
   E4m3Pages pages;
 };
 
@@ -157,144 +157,159 @@ __device__ __forceinline__ float over(float l) { return l == 0.f ? 0.f : 1.0f / 
 __device__ __forceinline__ float lse_of(float m, float l) { return l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l); }
 
 // ------------------------------------------------------------------------------------------ single tokens
-// One new token per sequence.  grid (runs, nkv * ceil(g / 16), B), block 64: a wave takes a run of tiles for up to 16 of the g heads
-// of a kv head and leaves unnormalised sums, maximum and denominator; a second kernel joins the runs in order.  How the tiles
-// are cut into runs depends on the token's own position only, so a token's result does not depend on what else the step holds.
-// A whole tile (16 KiB with heads of 128) is in registers while the one before it is worked on: codes take half the registers that
-// the numbers would.
-__host__ __device__ __forceinline__ int e4m3_tiles_per_run(int p) { return p >= 4096 ? 3 : 1; }
-__host__ __device__ __forceinline__ int e4m3_runs_at(int p) { return p / E4M3_TILE / e4m3_tiles_per_run(p) + 1; }
-static int e4m3_most_runs(int max_end) {
-  const int tiles = (max_end + E4M3_TILE - 1) / E4M3_TILE;
-  return max(min(tiles, 64), (tiles + 2) / 3) + 1;
-}
-
-template <int DT>
-struct TileCodes {
-  u32x4 k[4][DT / 4], v[DT];
-  f32x4 ks, vs;
-};
-template <int DT>
-__device__ __forceinline__ void fetch(TileCodes<DT>& t, const E4m3Pages& p, const int* row, int tile, int kvh) {
-  const int lane = threadIdx.x % 64, r = lane % 16, c = lane / 16;
-  int in_page;
-  int64_t head = e4m3_head_of(p, row, tile, kvh, in_page);
-  if (head < 0) head = 0;      // (no page: the host has checked that there is one)
-  const int64_t at = e4m3_tile_at(p, head, in_page), scales = e4m3_scale_at(p, head, in_page);
-  t.ks = *reinterpret_cast<const f32x4*>(p.k_scale + scales);
-  t.vs = *reinterpret_cast<const f32x4*>(p.v_scale + scales);
-  // (chunks behind the head's end: the last one again, against zeros of the query; dimensions behind it are not stored)
-#pragma unroll
-  for (int ks = 0; ks < DT / 4; ++ks) {
-    const int ch = min(4 * ks + c, p.hd / 16 - 1);
-#pragma unroll
-    for (int jt = 0; jt < 4; ++jt)
-      t.k[jt][ks] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p.k + at + ch * 1024 + (16 * jt + r) * 16));
-  }
-#pragma unroll
-  for (int dt = 0; dt < DT; ++dt) {
-    const int d = min(16 * dt, p.hd - 16) + r;
-    t.v[dt] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p.v + at + d * 64 + 16 * c));
-  }
+// One new token per sequence.  A wave takes tiles for up to 16 of the g heads of a kv head, run by run, and leaves a run's unnormalised
+// sums, maximum and denominator; the runs are then joined in order.  How the tiles are cut into runs depends on the token's own
+// position and on g only, so a token's result does not depend on what else the step holds.  Up to SHORT_END positions a workgroup does
+// it all, its waves' runs meeting in LDS: one launch.  Beyond, a wave streams through as many runs as make some thousands of
+// waves, and a second launch joins.
+// Bound by the bytes of the cache: 16 KiB of codes a tile with heads of 128.  A tile's keys are asked for as soon as the one before
+// has been multiplied, its values when that one's have: 64 registers hold what is on its way and what is worked on.
+// Runs leave g (hd + 2) numbers of 32 bits each, written and read again, for 128 hd bytes a tile: with more heads to a kv head they
+// are longer.
+#define SHORT_END 1024
+#define SHORT_WAVES 8
+__host__ __device__ __forceinline__ int e4m3_tiles_per_run(int p, int g) { return p < SHORT_END ? 1 : max(p < 4096 ? 1 : 3, min(4, (g + 1) / 2)); }
+__host__ __device__ __forceinline__ int e4m3_runs_at(int p, int g) { return p / E4M3_TILE / e4m3_tiles_per_run(p, g) + 1; }
+// Most runs of a token at a position below max_end.
+static int e4m3_most_runs(int max_end, int g) {
+  int most = 1;
+  const int ends[4] = {SHORT_END, 4096, max_end, 0};
+  for (int e : ends)
+    if (e > 0) most = max(most, e4m3_runs_at(min(e, max_end) - 1, g));
+  return most;
 }
 
 template <int DT, bool MOD>
-__global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(DT > 8 ? 1 : 2))) void e4m3_decode_kernel(E4m3Attn a) {
-  const int b = blockIdx.z, g = a.nh / a.nkv, ngc = (g + 15) / 16, kvh = blockIdx.y / ngc, cg = blockIdx.y % ngc;
-  const int lane = threadIdx.x, r = lane % 16, c = lane / 16, hd = a.pages.hd;
-  const int p = a.start[b], lo = reach_lo(p, a.window, a.mod.chunk);
-  const int S = e4m3_tiles_per_run(p), n_runs = e4m3_runs_at(p);
-  if ((int)blockIdx.x >= n_runs) return;
-  const bool valid = cg * 16 + r < g;
-  const int h = kvh * g + (valid ? cg * 16 + r : 0);
-  const int* row = a.pages.table + (int64_t)a.slots[b] * a.pages.bt_stride;
-  const float r1 = MOD && a.mod.r1 ? a.mod.r1[h] : 0.f, r2 = MOD && a.mod.r1 ? a.mod.r2[h] : 0.f;
+struct DecodeWave {
+  const E4m3Attn& a;
+  const int* row;
+  int kvh, p, lo, h, r, c;
+  bool valid;
+  float r1, r2;
   bf16x8 qf[2 * (DT / 4)][PIECES];
-  const act_t* qrow = a.q + ((int64_t)a.cu[b] * a.nh + h) * hd;
+  u32x4 k[4][DT / 4], v[DT];
+  f32x4 ks, vs;
+  f32x4 o[DT];
+  float m, l;
+
+  __device__ __forceinline__ DecodeWave(const E4m3Attn& args, int b, int kv, int cg) : a(args), kvh(kv) {
+    const int lane = threadIdx.x % 64, g = a.nh / a.nkv, hd = a.pages.hd;
+    r = lane % 16;
+    c = lane / 16;
+    p = a.start[b];
+    lo = reach_lo(p, a.window, a.mod.chunk);
+    valid = cg * 16 + r < g;
+    h = kvh * g + (valid ? cg * 16 + r : 0);
+    row = a.pages.table + (int64_t)a.slots[b] * a.pages.bt_stride;
+    r1 = MOD && a.mod.r1 ? a.mod.r1[h] : 0.f;
+    r2 = MOD && a.mod.r1 ? a.mod.r2[h] : 0.f;
+    const act_t* qrow = a.q + ((int64_t)a.cu[b] * a.nh + h) * hd;
 #pragma unroll
-  for (int ks = 0; ks < DT / 4; ++ks)
+    for (int s = 0; s < DT / 4; ++s)
 #pragma unroll
-    for (int half = 0; half < 2; ++half) load_query(qf[2 * ks + half], qrow, 64 * ks + 16 * c + 8 * half, hd, valid);
-  for (int run = blockIdx.x; run < n_runs; run += gridDim.x) {
-    const int beg = max(run * S, lo / E4M3_TILE), end = min((run + 1) * S, p / E4M3_TILE + 1);
-    if (beg >= end) continue;
-    f32x4 o[DT];
+      for (int half = 0; half < 2; ++half) load_query(qf[2 * s + half], qrow, 64 * s + 16 * c + 8 * half, hd, valid);
+    clear();
+  }
+  __device__ __forceinline__ void clear() {
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) o[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
-    float m = -INFINITY, l = 0.f;
-    auto step = [&](const TileCodes<DT>& t, int tile) {
-      const int pos0 = tile * E4M3_TILE;
-      f32x4 s[4];
+    m = -INFINITY;
+    l = 0.f;
+  }
+  __device__ __forceinline__ int64_t place(int tile, int64_t& scales) const {
+    int in_page;
+    int64_t head = e4m3_head_of(a.pages, row, tile, kvh, in_page);
+    if (head < 0) head = 0;      // (no page: the host has checked that there is one)
+    scales = e4m3_scale_at(a.pages, head, in_page);
+    return e4m3_tile_at(a.pages, head, in_page);
+  }
+  // (chunks behind the head's end: the last one again, against zeros of the query; dimensions behind it are not stored)
+  __device__ __forceinline__ void fetch_k(int tile) {
+    int64_t scales;
+    const uint8_t* at = a.pages.k + place(tile, scales);
+    ks = *reinterpret_cast<const f32x4*>(a.pages.k_scale + scales);
 #pragma unroll
-      for (int jt = 0; jt < 4; ++jt) {
-        s[jt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < DT / 4; ++s) {
+      const int ch = min(4 * s + c, a.pages.hd / 16 - 1);
 #pragma unroll
-        for (int ks = 0; ks < DT / 4; ++ks)
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const bf16x8 kf = numbers(t.k[jt][ks][2 * half], t.k[jt][ks][2 * half + 1], t.ks[jt]);
-#pragma unroll
-            for (int pc = PIECES - 1; pc >= 0; --pc)
-              s[jt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[2 * ks + half][pc], s[jt], 0, 0, 0);
-          }
-      }
-      final_scores<MOD>(s, a, r1, r2, pos0, p, lo, pos0 + E4M3_TILE - 1 > p || pos0 < lo);
-      if (a.scores && valid) {
-        float* at = a.scores + ((int64_t)b * a.nh + h) * a.ld_scores + pos0 + 4 * c;
-#pragma unroll
-        for (int jt = 0; jt < 4; ++jt) *reinterpret_cast<f32x4*>(at + 16 * jt) = s[jt];
-      }
-      bf16x8 pf[2][PIECES];
-      softmax_tile<DT>(s, o, m, l, pf);
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-        for (int pr = 0; pr < 2; ++pr) {
-          const bf16x8 lo8 = numbers(t.v[dt][2 * pr], t.v[dt][2 * pr], t.vs[2 * pr]);
-          const bf16x8 hi8 = numbers(t.v[dt][2 * pr + 1], t.v[dt][2 * pr + 1], t.vs[2 * pr + 1]);
-          const bf16x8 vf = __builtin_shufflevector(lo8, hi8, 0, 1, 2, 3, 8, 9, 10, 11);
-#pragma unroll
-          for (int pc = PIECES - 1; pc >= 0; --pc) o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[pr][pc], o[dt], 0, 0, 0);
-        }
-    };
-    TileCodes<DT> t0, t1;
-    fetch<DT>(t0, a.pages, row, beg, kvh);
-    for (int tile = beg; tile < end; tile += 2) {
-      if (tile + 1 < end) fetch<DT>(t1, a.pages, row, tile + 1, kvh);
-      step(t0, tile);
-      if (tile + 1 < end) {
-        if (tile + 2 < end) fetch<DT>(t0, a.pages, row, tile + 2, kvh);
-        step(t1, tile + 1);
-      }
-    }
-    if (!valid) continue;
-    float* out = a.partial + (((int64_t)b * a.nh + h) * a.max_runs + run) * (hd + 2);
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt)
-      if (16 * dt < hd)
-#pragma unroll
-        for (int v = 0; v < 4; ++v) out[16 * dt + 4 * c + v] = o[dt][v];
-    if (c == 0) {
-      out[hd] = m;
-      out[hd + 1] = l;
+      for (int jt = 0; jt < 4; ++jt)
+        k[jt][s] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(at + (uint32_t)(ch * 1024 + (16 * jt + r) * 16)));
     }
   }
-}
+  __device__ __forceinline__ void fetch_v(int tile) {
+    int64_t scales;
+    const uint8_t* at = a.pages.v + place(tile, scales);
+    vs = *reinterpret_cast<const f32x4*>(a.pages.v_scale + scales);
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+      v[dt] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(at + (uint32_t)((min(16 * dt, a.pages.hd - 16) + r) * 64 + 16 * c)));
+  }
+  // One tile; `next`, if there is one, is asked for meanwhile.
+  __device__ __forceinline__ void step(int b, int tile, int next) {
+    const int pos0 = tile * E4M3_TILE;
+    f32x4 s[4];
+#pragma unroll
+    for (int jt = 0; jt < 4; ++jt) {
+      s[jt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < DT / 4; ++i)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const bf16x8 kf = numbers(k[jt][i][2 * half], k[jt][i][2 * half + 1], ks[jt]);
+#pragma unroll
+          for (int pc = PIECES - 1; pc >= 0; --pc)
+            s[jt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[2 * i + half][pc], s[jt], 0, 0, 0);
+        }
+    }
+    if (next >= 0) fetch_k(next);
+    final_scores<MOD>(s, a, r1, r2, pos0, p, lo, pos0 + E4M3_TILE - 1 > p || pos0 < lo);
+    if (a.scores && valid) {
+      float* at = a.scores + ((int64_t)b * a.nh + h) * a.ld_scores + pos0 + 4 * c;
+#pragma unroll
+      for (int jt = 0; jt < 4; ++jt) *reinterpret_cast<f32x4*>(at + 16 * jt) = s[jt];
+    }
+    bf16x8 pf[2][PIECES];
+    softmax_tile<DT>(s, o, m, l, pf);
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int pr = 0; pr < 2; ++pr) {
+        const bf16x8 x = numbers(v[dt][2 * pr], v[dt][2 * pr], vs[2 * pr]), y = numbers(v[dt][2 * pr + 1], v[dt][2 * pr + 1], vs[2 * pr + 1]);
+        const bf16x8 vf = __builtin_shufflevector(x, y, 0, 1, 2, 3, 8, 9, 10, 11);
+#pragma unroll
+        for (int pc = PIECES - 1; pc >= 0; --pc) o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[pr][pc], o[dt], 0, 0, 0);
+      }
+    if (next >= 0) fetch_v(next);
+  }
+  // A run's sums to its place, and a new run.
+  __device__ __forceinline__ void leave(float* out) {
+    if (valid) {
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+        if (16 * dt < a.pages.hd)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) out[16 * dt + 4 * c + e] = o[dt][e];
+      if (c == 0) {
+        out[a.pages.hd] = m;
+        out[a.pages.hd + 1] = l;
+      }
+    }
+    clear();
+  }
+};
 
-// Joins the runs of one (sequence, head) in order: grid (nh, B), a wave to every 64 dimensions, each working out the runs' weights
-// for itself, 64 runs at a time.
-__global__ __launch_bounds__(256) void e4m3_join_kernel(E4m3Attn a) {
-  const int h = blockIdx.x, b = blockIdx.y, lane = threadIdx.x % 64, hd = a.pages.hd;
-  const int p = a.start[b], lo = reach_lo(p, a.window, a.mod.chunk), S = e4m3_tiles_per_run(p);
-  const int beg = lo / E4M3_TILE / S, end = p / E4M3_TILE / S + 1, stride = hd + 2;
-  const float* part = a.partial + ((int64_t)b * a.nh + h) * a.max_runs * stride;
+// One wave joins the runs [beg, end) of one head, `stride` numbers apart, and writes the output row; gives log2 of the row's sum.
+// Denominators are added 64 runs at a time, sums in four strands by run, which are added at the end.  `mine`: the strand of a wave
+// that shares the head with three others (their strands meet in `strands`, [4][256]), or -1: all four.
+template <int MINE>
+__device__ __forceinline__ float join_runs(const E4m3Attn& a, const float* part, int stride, int beg, int end, int h, int64_t t, int mine, float* strands) {
+  const int lane = threadIdx.x % 64, hd = a.pages.hd;
   float m = a.mod.sink ? a.mod.sink[h] * LOG2E : -INFINITY;
   for (int i = beg + lane; i < end; i += 64) m = fmaxf(m, part[(int64_t)i * stride + hd]);
   m = wave_max(m);
   const float use = m == -INFINITY ? 0.f : m;
   float l = a.mod.sink ? __builtin_amdgcn_exp2f(a.mod.sink[h] * LOG2E - use) : 0.f;
-  const int d = threadIdx.x;
-  float acc = 0.f;
+  float acc[MINE == 0 ? 4 : 1][4] = {};
   for (int i0 = beg; i0 < end; i0 += 64) {
     const int i = i0 + lane;
     float w = 0.f, wl = 0.f;
@@ -304,31 +319,132 @@ __global__ __launch_bounds__(256) void e4m3_join_kernel(E4m3Attn a) {
     }
     l += wave_sum(wl);
     const int n = min(64, end - i0);
-#pragma unroll 8
-    for (int j = 0; j < n; ++j) {
-      const float wj = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), j));
-      if (d < hd) acc = fmaf(wj, part[(int64_t)(i0 + j) * stride + d], acc);
+#pragma unroll(MINE == 0 ? 2 : 8)
+    for (int j = MINE == 0 ? 0 : mine; j < n; j += 4) {
+#pragma unroll
+      for (int s = 0; s < (MINE == 0 ? 4 : 1); ++s) {
+        if (j + s >= n) break;
+        const float ws = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), j + s));
+        const float* from = part + (int64_t)(i0 + j + s) * stride;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (64 * e < hd) acc[s][e] = fmaf(ws, from[min(64 * e + lane, hd - 1)], acc[s][e]);
+      }
     }
   }
-  const int64_t t = a.cu[b];
-  if (d < hd) a.out[(t * a.nh + h) * hd + d] = from_f32<act_t>(acc * over(l));
-  if (a.lse && d == 0) a.lse[t * a.nh + h] = lse_of(m, l);
+  const float inv = over(l);
+  act_t* out = a.out + (t * a.nh + h) * hd;
+  if constexpr (MINE != 0) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) strands[256 * mine + 64 * e + lane] = acc[0][e];
+    __syncthreads();
+    const int d = threadIdx.x;
+    if (d < hd) out[d] = from_f32<act_t>(((strands[d] + strands[256 + d]) + (strands[512 + d] + strands[768 + d])) * inv);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (64 * e + lane < hd) out[64 * e + lane] = from_f32<act_t>(((acc[0][e] + acc[1][e]) + (acc[2][e] + acc[3][e])) * inv);
+  }
+  return lse_of(m, l);
 }
-
-// The weights that a step of single tokens gives its positions: grid (tiles of 256 positions, nkv, B), a thread to a position.
-__global__ __launch_bounds__(256) void e4m3_decode_weights_kernel(E4m3Attn a) {
-  const int j = blockIdx.x * 256 + threadIdx.x, kvh = blockIdx.y, b = blockIdx.z, g = a.nh / a.nkv;
-  const int p = a.start[b], lo = reach_lo(p, a.window, a.mod.chunk);
-  if (j > p || j < lo) return;
+// log2 of a row's sum alone, as join_runs gives it.
+__device__ __forceinline__ float lse_of_runs(const E4m3Attn& a, const float* part, int stride, int beg, int end, int h) {
+  const int lane = threadIdx.x % 64, hd = a.pages.hd;
+  float m = a.mod.sink ? a.mod.sink[h] * LOG2E : -INFINITY;
+  for (int i = beg + lane; i < end; i += 64) m = fmaxf(m, part[(int64_t)i * stride + hd]);
+  m = wave_max(m);
+  const float use = m == -INFINITY ? 0.f : m;
+  float l = a.mod.sink ? __builtin_amdgcn_exp2f(a.mod.sink[h] * LOG2E - use) : 0.f;
+  for (int i0 = beg; i0 < end; i0 += 64) {
+    const int i = i0 + lane;
+    l += wave_sum(i < end ? __builtin_amdgcn_exp2f(part[(int64_t)i * stride + hd] - use) * part[(int64_t)i * stride + hd + 1] : 0.f);
+  }
+  return lse_of(m, l);
+}
+// A position's weight of one token: the sum over the g heads of a kv head, whose sums `lse` has.
+__device__ __forceinline__ void add_weight(const E4m3Attn& a, const int* row, int b, int kvh, int j, const float* lse) {
+  const int g = a.nh / a.nkv;
   int in_page;
-  const int64_t head = e4m3_head_of(a.pages, a.pages.table + (int64_t)a.slots[b] * a.pages.bt_stride, j / E4M3_TILE, kvh, in_page);
+  const int64_t head = e4m3_head_of(a.pages, row, j / E4M3_TILE, kvh, in_page);
   if (head < 0) return;
   float w = 0.f;
-  for (int i = 0; i < g; ++i) {
-    const int h = kvh * g + i;
-    w += __builtin_amdgcn_exp2f(a.scores[((int64_t)b * a.nh + h) * a.ld_scores + j] - a.lse[(int64_t)a.cu[b] * a.nh + h]);
-  }
+  for (int i = 0; i < g; ++i)
+    w += __builtin_amdgcn_exp2f(a.scores[((int64_t)b * a.nh + kvh * g + i) * a.ld_scores + j] - lse[i]);
   a.pages.weight[head * a.pages.page_size + in_page * E4M3_TILE + j % E4M3_TILE] += w;
+}
+
+// Runs of all but the shortest sequences: grid (waves, nkv * ceil(g / 16), B), block 64; a wave streams through neighbouring runs.
+template <int DT, bool MOD>
+__global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(DT > 12 || DT * PIECES > 24 ? 1 : DT * PIECES > 8 ? 2 : 3))) void e4m3_decode_kernel(E4m3Attn a) {
+  const int b = blockIdx.z, g = a.nh / a.nkv, ngc = (g + 15) / 16;
+  const int p = a.start[b], S = e4m3_tiles_per_run(p, g), lo = reach_lo(p, a.window, a.mod.chunk);
+  const int first_run = lo / E4M3_TILE / S, n_runs = e4m3_runs_at(p, g) - first_run, each = (n_runs + (int)gridDim.x - 1) / (int)gridDim.x;
+  const int run0 = first_run + (int)blockIdx.x * each, run1 = min(run0 + each, first_run + n_runs);
+  if (run0 >= run1) return;
+  DecodeWave<DT, MOD> w(a, b, blockIdx.y / ngc, blockIdx.y % ngc);
+  const int beg = max(run0 * S, lo / E4M3_TILE), end = min(run1 * S, p / E4M3_TILE + 1);
+  float* out = a.partial + ((int64_t)b * a.nh + w.h) * a.max_runs * (a.pages.hd + 2);
+  w.fetch_k(beg);
+  w.fetch_v(beg);
+  for (int tile = beg; tile < end; ++tile) {
+    w.step(b, tile, tile + 1 < end ? tile + 1 : -1);
+    if ((tile + 1) % S == 0 || tile + 1 == end) w.leave(out + (int64_t)(tile / S) * (a.pages.hd + 2));
+  }
+}
+
+// Joins them: blocks 0 .. nh B - 1 a head each, four waves with a strand of its runs each; behind them, with weights, blocks of 256 positions of
+// one (sequence, kv head), which work the heads' sums out for themselves.
+__global__ __launch_bounds__(256) void e4m3_join_kernel(E4m3Attn a, int blocks_of_weights) {
+  __shared__ float lds[4 * 256];
+  const int stride = a.pages.hd + 2, g = a.nh / a.nkv, wave = threadIdx.x / 64, lane = threadIdx.x % 64;
+  const bool joins = (int)blockIdx.x < a.nh * a.B;
+  const int x = joins ? (int)blockIdx.x : (int)blockIdx.x - a.nh * a.B;
+  const int b = joins ? x / a.nh : x / blocks_of_weights / a.nkv;
+  const int p = a.start[b], lo = reach_lo(p, a.window, a.mod.chunk), S = e4m3_tiles_per_run(p, g);
+  const int beg = lo / E4M3_TILE / S, end = p / E4M3_TILE / S + 1;
+  if (joins) {
+    const int h = x % a.nh;
+    join_runs<1>(a, a.partial + ((int64_t)b * a.nh + h) * a.max_runs * stride, stride, beg, end, h, a.cu[b], wave, lds);
+    return;
+  }
+  const int kvh = x / blocks_of_weights % a.nkv, j = x % blocks_of_weights * 256 + (int)threadIdx.x;
+  if (j - (int)threadIdx.x > p || j - (int)threadIdx.x + 255 < lo) return;
+  const int* row = a.pages.table + (int64_t)a.slots[b] * a.pages.bt_stride;
+  for (int i = wave; i < g; i += 4) {      // (at most 1,024 heads to a kv head: the launcher has checked)
+    const int h = kvh * g + i;
+    const float lse = lse_of_runs(a, a.partial + ((int64_t)b * a.nh + h) * a.max_runs * stride, stride, beg, end, h);
+    if (lane == 0) lds[i] = lse;
+  }
+  __syncthreads();
+  if (j >= lo && j <= p) add_weight(a, row, b, kvh, j, lds);
+}
+
+// A step whose sequences all hold at most SHORT_END positions: grid (nkv * ceil(g / 16), B), one launch.
+template <int DT, bool MOD>
+__global__ __launch_bounds__(64 * SHORT_WAVES) __attribute__((amdgpu_waves_per_eu(DT * PIECES > 8 ? 1 : 2))) void e4m3_short_kernel(E4m3Attn a) {
+  extern __shared__ float sums[];      // [runs][heads of the workgroup][hd + 2]
+  __shared__ float lse[16];
+  const int b = blockIdx.y, g = a.nh / a.nkv, ngc = (g + 15) / 16, kvh = blockIdx.x / ngc, cg = blockIdx.x % ngc;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64, stride = a.pages.hd + 2, heads = min(16, g - 16 * cg);
+  DecodeWave<DT, MOD> w(a, b, kvh, cg);
+  const int beg = w.lo / E4M3_TILE, end = w.p / E4M3_TILE + 1;
+  if (beg + wave < end) {
+    w.fetch_k(beg + wave);
+    w.fetch_v(beg + wave);
+  }
+  for (int tile = beg + wave; tile < end; tile += SHORT_WAVES) {
+    w.step(b, tile, tile + SHORT_WAVES < end ? tile + SHORT_WAVES : -1);
+    w.leave(sums + ((tile - beg) * heads + min(w.r, heads - 1)) * stride);
+  }
+  __syncthreads();
+  for (int i = wave; i < heads; i += SHORT_WAVES) {
+    const float x = join_runs<0>(a, sums + i * stride, heads * stride, 0, end - beg, kvh * g + 16 * cg + i, a.cu[b], -1, nullptr);
+    if (lane == 0) lse[i] = x;
+  }
+  if (!a.scores) return;
+  __threadfence_block();      // (the scores that the workgroup's waves have written)
+  __syncthreads();
+  for (int j = max(w.lo, beg * E4M3_TILE) + (int)threadIdx.x; j <= w.p; j += 64 * SHORT_WAVES) add_weight(a, w.row, b, kvh, j, lse);
 }
 
 // ------------------------------------------------------------------------------------------ prompts
@@ -483,6 +599,26 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DT > 8 ? 1 
   }
 }
 
+template <int DT>
+struct TileKeys {
+  u32x4 k[4][DT / 4];
+  f32x4 ks;
+};
+template <int DT>
+__device__ __forceinline__ void fetch_keys(TileKeys<DT>& t, const E4m3Pages& p, const int* row, int tile, int kvh) {
+  const int lane = threadIdx.x % 64, r = lane % 16, c = lane / 16;
+  int in_page;
+  int64_t head = e4m3_head_of(p, row, tile, kvh, in_page);
+  if (head < 0) head = 0;
+  const uint8_t* at = p.k + e4m3_tile_at(p, head, in_page);
+  t.ks = *reinterpret_cast<const f32x4*>(p.k_scale + e4m3_scale_at(p, head, in_page));
+#pragma unroll
+  for (int ks = 0; ks < DT / 4; ++ks) {
+    const int ch = min(4 * ks + c, p.hd / 16 - 1);
+#pragma unroll
+    for (int jt = 0; jt < 4; ++jt) t.k[jt][ks] = *reinterpret_cast<const u32x4*>(at + ch * 1024 + (16 * jt + r) * 16);
+  }
+}
 // The weights that a prompt gives its positions, from the scores once more and the rows' sums: grid (tiles, nkv, B), block 256.  A
 // workgroup keeps a tile's keys in registers and goes through the tokens that may see it and the heads of its kv head, 16 tokens of one
 // head to a wave at a time; one sum over lanes and waves at the end, in a fixed order.
@@ -494,9 +630,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DT > 8 ? 1 
   const int t0 = a.cu[b], n = a.cu[b + 1] - t0, start = a.start[b];
   const int tile = reach_lo(start, a.window, a.mod.chunk) / E4M3_TILE + (int)blockIdx.x, pos0 = tile * E4M3_TILE;
   if (n <= 0 || pos0 >= start + n) return;
-  TileCodes<DT> t;
+  TileKeys<DT> t;
   const int* row = a.pages.table + (int64_t)a.slots[b] * a.pages.bt_stride;
-  fetch<DT>(t, a.pages, row, tile, kvh);
+  fetch_keys<DT>(t, a.pages, row, tile, kvh);
   // the tokens that may see a position of the tile: from the tile's first to the last whose reach has its last
   const int from = max(pos0 - start, 0) / 16;
   int to = n;
@@ -552,12 +688,22 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DT > 8 ? 1 
 }
 
 // ------------------------------------------------------------------------------------------ launch
+#define DECODE_WAVES 4096      // waves of a step beyond which a wave takes more runs instead
 template <int DT, bool MOD>
 static int launch_decode(const E4m3Attn& a, int max_end, hipStream_t st) {
-  const int g = a.nh / a.nkv;
-  hipLaunchKernelGGL((e4m3_decode_kernel<DT, MOD>), dim3(e4m3_runs_at(max_end > 0 ? max_end - 1 : 0), a.nkv * ((g + 15) / 16), a.B), dim3(64), 0, st, a);
-  hipLaunchKernelGGL(e4m3_join_kernel, dim3(a.nh, a.B), dim3((a.pages.hd + 63) / 64 * 64), 0, st, a);
-  if (a.scores) hipLaunchKernelGGL(e4m3_decode_weights_kernel, dim3((max_end + 255) / 256, a.nkv, a.B), dim3(256), 0, st, a);
+  const int g = a.nh / a.nkv, columns = a.nkv * ((g + 15) / 16);
+  if constexpr (DT <= 12 && DT * PIECES <= 24) {      // (wider heads: two waves to a SIMD have too few registers)
+    const size_t shmem = (size_t)((max_end + E4M3_TILE - 1) / E4M3_TILE) * g * (a.pages.hd + 2) * sizeof(float);
+    if (max_end <= SHORT_END && g <= 16 && shmem <= 64 * 1024) {
+      hipLaunchKernelGGL((e4m3_short_kernel<DT, MOD>), dim3(columns, a.B), dim3(64 * SHORT_WAVES), shmem, st, a);
+      return 0;
+    }
+  }
+  const int waves = min(a.max_runs, max(1, DECODE_WAVES / (columns * a.B)));
+  hipLaunchKernelGGL((e4m3_decode_kernel<DT, MOD>), dim3(waves, columns, a.B), dim3(64), 0, st, a);
+  const int blocks = a.scores ? (max_end + 255) / 256 : 0;
+  if ((int64_t)a.nh * a.B + (int64_t)blocks * a.nkv * a.B > 0xFFFFFF) return TQ_ERR_UNSUPPORTED;
+  hipLaunchKernelGGL(e4m3_join_kernel, dim3(a.nh * a.B + blocks * a.nkv * a.B), dim3(256), 0, st, a, blocks);
   return 0;
 }
 template <int DT, int QG, bool MOD>
@@ -586,12 +732,12 @@ static int launch(const E4m3Attn& a, int decode, int max_new, int max_end, hipSt
   return a.mod.cap > 0.f || a.mod.r1 ? launch_as<DT, true>(a, decode, max_new, max_end, st) : launch_as<DT, false>(a, decode, max_new, max_end, st);
 }
 
-// Floats of scratch: for decoding the runs' sums, with weights the scores and the rows' sums too; for prompts with weights the rows' sums.
-TQ_API int64_t tq_e4m3_attention_scratch(int T, int B, int nh, int hd, int max_end, int decode, int weights) {
+// Floats of scratch: for decoding the runs' sums, with weights the scores too; for prompts with weights the rows' sums.
+TQ_API int64_t tq_e4m3_attention_scratch(int T, int B, int nh, int nkv, int hd, int max_end, int decode, int weights) {
   const int64_t rows = weights ? (int64_t)T * nh : 0;
   if (!decode) return rows;
   const int64_t ld = (max_end + E4M3_TILE - 1) / E4M3_TILE * E4M3_TILE;
-  return (int64_t)B * nh * e4m3_most_runs(max_end) * (hd + 2) + (weights ? (int64_t)B * nh * ld : 0) + rows + 4;
+  return (int64_t)B * nh * e4m3_most_runs(max_end, nh / nkv) * (hd + 2) + (weights ? (int64_t)B * nh * ld : 0);
 }
 
 // q, out [T][nh][hd]; tokens as runs (cu, slots, start) whose keys and values the cache holds already.  decode != 0: one token per
@@ -603,10 +749,10 @@ TQ_API int tq_e4m3_attention(const void* q, void* out, const int* cu, const int*
                              int max_end, hipStream_t st) {
   if (B <= 0 || T <= 0) return 0;
   if ((r1 == nullptr) != (r2 == nullptr) || chunk < 0 || softcap < 0.f || window < 0 || nh <= 0 || max_new <= 0 || max_end <= 0) return TQ_ERR_BAD_ARG;
-  if (!e4m3_pages_fit(page_size, heads, head0, nkv, hd) || nh % nkv != 0 || nh > 65535 || B > 65535) return TQ_ERR_UNSUPPORTED;
+  if (!e4m3_pages_fit(page_size, heads, head0, nkv, hd) || nh % nkv != 0 || nh > 65535 || nh / nkv > 1024 || B > 65535) return TQ_ERR_UNSUPPORTED;
   if ((decode || weight) && !scratch) return TQ_ERR_BAD_ARG;
   E4m3Attn a{(const act_t*)q, (act_t*)out, cu, slots, start, B, nh, nkv, window, scale, ScoreMod{softcap, r1, r2, chunk, sink, nullptr, 0},
-             nullptr, e4m3_most_runs(max_end), nullptr, 0, nullptr,
+             nullptr, e4m3_most_runs(max_end, nh / nkv), nullptr, 0, nullptr,
              E4m3Pages{(uint8_t*)k, (uint8_t*)v, (float*)k_scale, (float*)v_scale, weight, table, bt_stride, page_size, heads, head0, hd}};
   if (decode) {
     // (the scores first: their rows are read and written 16 bytes at a time)
@@ -616,9 +762,9 @@ TQ_API int tq_e4m3_attention(const void* q, void* out, const int* cu, const int*
       scratch += (int64_t)B * nh * a.ld_scores;
     }
     a.partial = scratch;
-    scratch += (int64_t)B * nh * a.max_runs * (hd + 2);
+  } else if (weight) {
+    a.lse = scratch;
   }
-  if (weight) a.lse = scratch;
   const int dt = hd / 16;
   const int rc = dt <= 4 ? launch<4>(a, decode, max_new, max_end, st) : dt <= 8 ? launch<8>(a, decode, max_new, max_end, st)
                : dt <= 12 ? launch<12>(a, decode, max_new, max_end, st) : launch<16>(a, decode, max_new, max_end, st);

@@ -17,193 +17,261 @@ struct E4m3Write {
   act_t* q;                     // [T][nh * hd]
   int T, B, nh, nkv, hd;
   int tiles;                    // most tiles that a sequence's new tokens touch
+  int kv_heads;                 // kv heads that a workgroup of keys and values goes through, one after the other
   int q_tokens, q_heads;        // tokens and heads of a workgroup of queries
   E4m3Pages pages;
   int write;
 };
+#define WRITE_THREADS 512
+#define WRITE_HEADS 8             // most kv heads of a workgroup
 
 __device__ __forceinline__ float bias_at(const E4m3Write& a, int i) {
   return a.bias_type == TQ_BF16 ? to_f32(((const bf16_t*)a.bias)[i]) : ((const float*)a.bias)[i];
 }
-// Sine and cosine of the exact product p * f: the rounded product's, turned on by the small angle that the rounding left out (positions
-// of a long cache: at 100,000 the rounded product of a fast pair is off by up to 0.004).
-__device__ __forceinline__ void turn_of(int p, float f, float amp, float& cs, float& sn) {
-  const float pf = (float)p, hi = pf * f, lo = fmaf(pf, f, -hi);
-  float s, c;
-  sincosf(hi, &s, &c);
-  const float l2 = lo * lo, ls = lo * fmaf(l2, -1.f / 6.f, 1.f), lc = l2 * fmaf(l2, 1.f / 24.f, -0.5f);      // sin lo, cos lo - 1
-  sn = amp * (s + fmaf(c, ls, s * lc));
-  cs = amp * (c + fmaf(-s, ls, c * lc));
+// (numbers col .. col + 3 of a token whose row begins `at` numbers behind `base`: 32 bits of offset from an address that all lanes share)
+__device__ __forceinline__ float4 four_at(const E4m3Write& a, const float* base, uint32_t at, int col) {
+  float4 v = *reinterpret_cast<const float4*>(base + (at + (uint32_t)col));
+  if (a.bias) v = make_float4(v.x + bias_at(a, col), v.y + bias_at(a, col + 1), v.z + bias_at(a, col + 2), v.w + bias_at(a, col + 3));
+  return v;
+}
+// Sine and cosine of the exact product p * f (48 bits, which 64-bit numbers hold), in 64 bits: reduced to an eighth of a turn about the
+// nearest quarter, then the series of sine and cosine, whose first omitted terms are r^13 / 13! and r^12 / 12! (1e-10 and less).  In 32
+// bits the product alone would be off by 0.004 at position 100,000, and the keys' codes would differ from exact ones more often than
+// rounding makes them (with 1 ulp of error in the sine, 1.5 times as far from 64 bits as correctly rounded sines).
+__device__ __forceinline__ float2 turn_of(int p, float f, float amp) {
+  const double x = (double)p * (double)f, k = rint(x * 0.63661977236758134308);      // 2 / pi
+  const double r = fma(k, -6.123233995736766036e-17, fma(k, -1.5707963267948965580, x)), z = r * r;      // pi / 2 in two parts
+  const double s = r * (1. + z * (-1. / 6 + z * (1. / 120 + z * (-1. / 5040 + z * (1. / 362880 + z * (-1. / 39916800))))));
+  const double c = 1. + z * (-0.5 + z * (1. / 24 + z * (-1. / 720 + z * (1. / 40320 + z * (-1. / 3628800)))));
+  const int q = (int)((int64_t)k & 3);
+  const double cs = q == 0 ? c : q == 1 ? -s : q == 2 ? -c : s, sn = q == 0 ? s : q == 1 ? c : q == 2 ? -s : -c;
+  return make_float2(amp * (float)cs, amp * (float)sn);
+}
+// Four neighbouring numbers of a head from dimension d on, rotated; `turn`: the token's cosines and sines.  FOURS: four numbers rotate
+// alike (pairs by halves, a multiple of four of them, or neighbouring pairs, an even number of them).
+template <bool FOURS>
+__device__ __forceinline__ float4 rotated(const E4m3Write& a, const float* base, uint32_t at, int col, int d, const float2* turn) {
+  const int n = a.rot / 2;
+  const float4 x = four_at(a, base, at, col + d);
+  if (d >= 2 * n) return x;
+  if constexpr (FOURS) {
+    if (a.pairing == 1) {
+      const float2 t0 = turn[d / 2], t1 = turn[d / 2 + 1];
+      return make_float4(x.x * t0.x - x.y * t0.y, x.x * t0.y + x.y * t0.x, x.z * t1.x - x.w * t1.y, x.z * t1.y + x.w * t1.x);
+    }
+    const bool low = d < n;
+    const float4 y = four_at(a, base, at, col + (low ? d + n : d - n));
+    const float2* t = turn + (low ? d : d - n);
+    const float2 t0 = t[0], t1 = t[1], t2 = t[2], t3 = t[3];
+    const float f = low ? -1.f : 1.f;
+    return make_float4(x.x * t0.x + f * y.x * t0.y, x.y * t1.x + f * y.y * t1.y, x.z * t2.x + f * y.z * t2.y, x.w * t3.x + f * y.w * t3.y);
+  }
+  float o[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int e = d + j;
+    if (e < 2 * n) {
+      const bool low = a.pairing == 0 ? e < n : e % 2 == 0;
+      const int other = col + (a.pairing == 0 ? (low ? e + n : e - n) : e ^ 1);
+      const float y = base[at + (uint32_t)other] + (a.bias ? bias_at(a, other) : 0.f);
+      const float2 t = turn[a.pairing == 0 ? (low ? e : e - n) : e / 2];
+      o[j] = o[j] * t.x + (low ? -y : y) * t.y;
+    }
+  }
+  return make_float4(o[0], o[1], o[2], o[3]);
+}
+__device__ __forceinline__ float largest(float4 v) { return fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))); }
+__device__ __forceinline__ bool all_usable(float4 v) {
+  return fabsf(v.x) < E4M3_TOO_LARGE && fabsf(v.y) < E4M3_TOO_LARGE && fabsf(v.z) < E4M3_TOO_LARGE && fabsf(v.w) < E4M3_TOO_LARGE;
 }
 
-// A workgroup takes either one tile of 64 positions of one sequence and kv head (keys and values: a row that is not finite in one
-// is marked in both), or the queries of q_tokens tokens and q_heads heads.  Keys and values pass through LDS in 32 bits, where the
-// keys are rotated, since a block's scale has to be known before its first code.
+// A workgroup takes either one tile of 64 positions of one sequence and up to kv_heads kv heads in turn (keys and values: a row that is
+// not finite in one is marked in both), or the queries of q_tokens tokens and q_heads heads.  The tokens' cosines and sines are worked
+// out once and kept in LDS.  Every number is read once (keys and queries that rotate by halves: twice) and stays in registers until its block's
+// scale is known: a thread holds four neighbouring numbers of KI rows of keys, in an order that gives a wave rows of one block only,
+// and 16 positions of KI / 4 dimensions of values, the 16 codes that lie side by side in the page.
 // Bound by the bytes (a prompt) or by the launch (single tokens).
-__global__ __launch_bounds__(256) void e4m3_write_kernel(E4m3Write a) {
-  extern __shared__ __attribute__((aligned(16))) float lds[];
-  const int hd = a.hd, n = a.rot / 2, tid = threadIdx.x;
-  const int kv_groups = a.write ? a.tiles * a.nkv * a.B : 0;
+template <int KI, bool FOURS>
+__global__ __launch_bounds__(WRITE_THREADS) __attribute__((amdgpu_waves_per_eu(KI > 4 ? 2 : 4))) void e4m3_write_kernel(E4m3Write a) {
+  extern __shared__ __attribute__((aligned(16))) float2 turns[];
+  const int hd = a.hd, n = a.rot / 2, fours = hd / 4;
+  int tid = threadIdx.x;
+  const uint32_t ld = (uint32_t)a.ld;
+  const int kv_per = (a.nkv + a.kv_heads - 1) / max(a.kv_heads, 1), kv_groups = a.write ? a.tiles * kv_per * a.B : 0;
   if ((int)blockIdx.x >= kv_groups) {
-    // queries: the angles of the workgroup's tokens once, then four neighbouring numbers of a head at a time
     const int w = (int)blockIdx.x - kv_groups, per = (a.nh + a.q_heads - 1) / a.q_heads;
     const int t0 = w / per * a.q_tokens, h0 = w % per * a.q_heads;
     const int nt = min(a.q_tokens, a.T - t0), heads = min(a.q_heads, a.nh - h0);
-    float2* turn = reinterpret_cast<float2*>(lds);
-    for (int i = tid; i < nt * n; i += 256) {
-      float c, s;
-      turn_of(a.positions[t0 + i / n], a.inv_freq[i % n], a.amp, c, s);
-      turn[i] = make_float2(c, s);
-    }
+    for (int i = tid; i < nt * n; i += WRITE_THREADS) turns[i] = turn_of(a.positions[t0 + i / n], a.inv_freq[i % n], a.amp);
     __syncthreads();
-    const int fours = hd / 4, items = nt * heads * fours;
-    for (int i = tid; i < items; i += 256) {
-      const int d = i % fours * 4, h = h0 + i / fours % heads, t = i / (fours * heads);
-      const float* row = a.x + (int64_t)(t0 + t) * a.ld + (int64_t)h * hd;
-      float4 v = *reinterpret_cast<const float4*>(row + d);
-      float x[4] = {v.x, v.y, v.z, v.w}, o[4];
-      if (a.bias)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) x[j] += bias_at(a, h * hd + d + j);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int e = d + j;
-        o[j] = x[j];
-        if (e < 2 * n) {
-          const int pair = a.pairing == 0 ? (e < n ? e : e - n) : e / 2;
-          const bool low = a.pairing == 0 ? e < n : e % 2 == 0;
-          const int other = a.pairing == 0 ? (low ? e + n : e - n) : e ^ 1;
-          float y = a.pairing == 0 ? row[other] + (a.bias ? bias_at(a, h * hd + other) : 0.f) : x[j ^ 1];
-          const float2 cs = turn[t * n + pair];
-          o[j] = low ? x[j] * cs.x - y * cs.y : y * cs.y + x[j] * cs.x;
-        }
-      }
+    const int items = nt * heads * fours;
+    for (int i = tid; i < items; i += WRITE_THREADS) {
+      const int d = i % fours * 4, th = i / fours, h = h0 + th % heads, t = th / heads;
+      const float4 o = rotated<FOURS>(a, a.x + (int64_t)t0 * a.ld, (uint32_t)t * ld, h * hd, d, turns + t * n);
       act_t* out = a.q + ((int64_t)(t0 + t) * a.nh + h) * hd + d;
 #if defined(TQ_ACT_BF16)
-      *reinterpret_cast<uint2*>(out) = make_uint2(f32_to_bf16_pair(o[0], o[1]), f32_to_bf16_pair(o[2], o[3]));
+      *reinterpret_cast<uint2*>(out) = make_uint2(f32_to_bf16_pair(o.x, o.y), f32_to_bf16_pair(o.z, o.w));
 #else
-      *reinterpret_cast<float4*>(out) = make_float4(o[0], o[1], o[2], o[3]);
+      *reinterpret_cast<float4*>(out) = o;
 #endif
     }
     return;
   }
-  const int kvh = (int)blockIdx.x % a.nkv, b = (int)blockIdx.x / a.nkv % a.B, nth = (int)blockIdx.x / a.nkv / a.B;
+  constexpr int VI = KI / 4;
+  const int kvh0 = (int)blockIdx.x % kv_per * a.kv_heads, b = (int)blockIdx.x / kv_per % a.B, nth = (int)blockIdx.x / kv_per / a.B;
   const int t0 = a.cu[b], count = a.cu[b + 1] - t0, start = a.start[b];
   const int tile = start / E4M3_TILE + nth, pos0 = tile * E4M3_TILE;
   if (count <= 0 || pos0 >= start + count) return;
   const int r0 = max(start - pos0, 0), r1 = min(start + count - pos0, E4M3_TILE);      // the tile's rows that are new
   const int old0 = r0 / E4M3_BLOCK * E4M3_BLOCK;      // rows old0 .. r0 - 1 share the first new row's block
-  int in_page;
-  const int64_t head = e4m3_head_of(a.pages, a.pages.table + (int64_t)a.slots[b] * a.pages.bt_stride, tile, kvh, in_page);
-  if (head < 0) return;
-  const int stride = hd + 4;
-  float* K = lds;                                  // [64][hd + 4]
-  float* V = K + E4M3_TILE * stride;
-  __shared__ uint32_t top[2][4];
-  __shared__ int bad[E4M3_TILE];
-  __shared__ float inverse[2][4], ratio[2];
-  if (tid < 8) top[tid / 4][tid % 4] = 0u;
-  if (tid < E4M3_TILE) bad[tid] = 0;
-  const int rows = r1 - r0, fours = hd / 4;
-  const int64_t first = (int64_t)(t0 + pos0 + r0 - start);      // packed row of the tile's first new row
-  for (int i = tid; i < 2 * rows * fours; i += 256) {
-    const int d = i % fours * 4, m = i / fours % 2, r = i / (2 * fours);
-    const int col = (a.nh + m * a.nkv + kvh) * hd + d;
-    float4 v = *reinterpret_cast<const float4*>(a.x + (first + r) * a.ld + col);
-    if (a.bias) v = make_float4(v.x + bias_at(a, col), v.y + bias_at(a, col + 1), v.z + bias_at(a, col + 2), v.w + bias_at(a, col + 3));
-    *reinterpret_cast<float4*>((m ? V : K) + (r0 + r) * stride + d) = v;
-  }
+  __shared__ uint32_t top[WRITE_HEADS][2][4];         // the blocks' largest magnitudes, as bits
+  __shared__ uint32_t bad[WRITE_HEADS][2];            // rows that are not finite, a bit each
+  __shared__ float inverse[2][2][4], ratio[2][2];     // by turns, so that a wave may still read the last head's
+  for (int i = tid; i < WRITE_HEADS * 8; i += WRITE_THREADS) top[i / 8][i / 4 % 2][i % 4] = 0u;
+  if (tid < WRITE_HEADS * 2) bad[tid / 2][tid % 2] = 0u;
+  const int64_t first = (int64_t)t0 + pos0 - start;      // packed row of the tile's row 0 (rows before r0 are not read)
+  for (int i = tid; i < (r1 - r0) * n; i += WRITE_THREADS)
+    turns[i] = turn_of(a.positions[first + r0 + i / n], a.inv_freq[i % n], a.amp);
   __syncthreads();
-  for (int i = tid; i < rows * n; i += 256) {
-    const int pair = i % n, r = i / n;
-    const int lo = a.pairing == 0 ? pair : 2 * pair, hi = a.pairing == 0 ? pair + n : 2 * pair + 1;
-    float cs, sn;
-    turn_of(a.positions[first + r], a.inv_freq[pair], a.amp, cs, sn);
-    float* row = K + (r0 + r) * stride;
-    const float x = row[lo], y = row[hi];
-    row[lo] = x * cs - y * sn;
-    row[hi] = x * sn + y * cs;
-  }
-  __syncthreads();
-  // rows that are not finite, then the blocks' largest magnitudes without them
-  for (int i = tid; i < 2 * rows * fours; i += 256) {
-    const int d = i % fours * 4, m = i / fours % 2, r = r0 + i / (2 * fours);
-    const float4 v = *reinterpret_cast<const float4*>((m ? V : K) + r * stride + d);
-    if (!(fabsf(v.x) < E4M3_TOO_LARGE && fabsf(v.y) < E4M3_TOO_LARGE && fabsf(v.z) < E4M3_TOO_LARGE && fabsf(v.w) < E4M3_TOO_LARGE))
-      bad[r] = 1;
-  }
-  __syncthreads();
-  for (int i = tid; i < 2 * rows * fours; i += 256) {
-    const int d = i % fours * 4, m = i / fours % 2, r = r0 + i / (2 * fours);
-    if (bad[r]) continue;
-    const float4 v = *reinterpret_cast<const float4*>((m ? V : K) + r * stride + d);
-    atomicMax(&top[m][r / E4M3_BLOCK], __float_as_uint(fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w)))));
-  }
-  __syncthreads();
-  if (tid < 8) {
-    const int m = tid / 4, j = tid % 4;
-    if (j * E4M3_BLOCK < r1 && (j + 1) * E4M3_BLOCK > r0) {
-      float* at = (m ? a.pages.v_scale : a.pages.k_scale) + e4m3_scale_at(a.pages, head, in_page) + j;
-      float scale = e4m3_scale(__uint_as_float(top[m][j]));
-      if (j == r0 / E4M3_BLOCK) {
-        const float was = old0 < r0 ? *at : 0.f;
-        scale = fmaxf(scale, was);
-        ratio[m] = was * e4m3_inverse(scale);      // what the rows before the new ones are multiplied by (1: they stay)
+  const int lane = tid % 64;
+  const float* base = a.x + first * a.ld;
+#pragma unroll 1
+  for (int hi = 0; hi < a.kv_heads && kvh0 + hi < a.nkv; ++hi) {
+    // (places are worked out anew for every head: kept, they would be more registers than a wave has)
+    asm volatile("" : "+v"(tid));
+    const int kvh = kvh0 + hi;
+    int in_page;
+    const int64_t head = e4m3_head_of(a.pages, a.pages.table + (int64_t)a.slots[b] * a.pages.bt_stride, tile, kvh, in_page);
+    if (head < 0) return;      // (the same for every head of the tile)
+    const int kcol = (a.nh + kvh) * hd, vcol = (a.nh + a.nkv + kvh) * hd;
+    float4 k[KI];
+    float v[VI][16];
+#pragma unroll
+    for (int i = 0; i < KI; ++i) {
+      const int at = tid + i * WRITE_THREADS, r = at / fours;
+      k[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (r >= r0 && r < r1) k[i] = rotated<FOURS>(a, base, (uint32_t)r * ld, kcol, at % fours * 4, turns + (r - r0) * n);
+    }
+#pragma unroll
+    for (int i = 0; i < VI; ++i) {
+      const int at = tid + i * WRITE_THREADS, d = at % hd, c = at / hd;
+      const float add = a.bias && c < 4 ? bias_at(a, vcol + d) : 0.f;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const int r = 16 * (j / 4) + 4 * c + j % 4;
+        v[i][j] = c < 4 && r >= r0 && r < r1 ? (base + (int64_t)(16 * (j / 4) + j % 4) * a.ld)[(uint32_t)(4 * c) * ld + (uint32_t)(vcol + d)] + add : 0.f;
       }
-      *at = scale;
-      inverse[m][j] = e4m3_inverse(scale);
     }
-  }
-  __syncthreads();
-  uint8_t* kt = a.pages.k + e4m3_tile_at(a.pages, head, in_page);
-  uint8_t* vt = a.pages.v + e4m3_tile_at(a.pages, head, in_page);
-  const int from_k = ratio[0] != 1.f ? old0 : r0, from_v = ratio[1] != 1.f ? old0 : r0;
-  for (int i = tid; i < (r1 - from_k) * (hd / 16); i += 256) {
-    const int r = from_k + i % (r1 - from_k), ch = i / (r1 - from_k);
-    uint4* at = reinterpret_cast<uint4*>(kt + ch * 16 * E4M3_TILE + r * 16);
-    uint4 w;
-    if (r < r0) {
-      w = *at;
-      const float f = ratio[0];
-      w = make_uint4(e4m3_rescale(w.x, f, f, f, f), e4m3_rescale(w.y, f, f, f, f), e4m3_rescale(w.z, f, f, f, f), e4m3_rescale(w.w, f, f, f, f));
-    } else if (bad[r]) {
-      w = make_uint4(0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu);
-    } else {
-      const float f = inverse[0][r / E4M3_BLOCK];
-      const float4* row = reinterpret_cast<const float4*>(K + r * stride + ch * 16);
-      uint32_t c[4];
+    // largest magnitudes by block, and rows that are not finite
 #pragma unroll
-      for (int j = 0; j < 4; ++j) c[j] = e4m3_codes(row[j].x * f, row[j].y * f, row[j].z * f, row[j].w * f);
-      w = make_uint4(c[0], c[1], c[2], c[3]);
+    for (int i = 0; i < KI; ++i) {
+      const int r = (tid + i * WRITE_THREADS) / fours;
+      const float m = wave_max(largest(k[i]));
+      if (lane == 0 && r < E4M3_TILE) atomicMax(&top[hi][0][r / E4M3_BLOCK], __float_as_uint(m));
+      if (!all_usable(k[i])) atomicOr(&bad[hi][r / 32], 1u << r % 32);
     }
-    *at = w;
-  }
-  for (int i = tid; i < 16 * hd; i += 256) {
-    // four positions of one dimension: 16 j + 4 c ..
-    const int d = i % hd, j = i / hd / 4, c = i / hd % 4, p = 16 * j + 4 * c;
-    if (p >= r1 || p + 4 <= from_v) continue;
-    uint32_t* at = reinterpret_cast<uint32_t*>(vt + d * E4M3_TILE + 16 * c + 4 * j);
-    const bool whole = p >= r0 && p + 4 <= r1;
-    const uint32_t was = whole ? 0u : *at;
-    float x[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) x[e] = p + e >= r0 && p + e < r1 && !bad[p + e] ? V[(p + e) * stride + d] * inverse[1][j] : 0.f;
-    uint32_t w = e4m3_codes(x[0], x[1], x[2], x[3]);
-    if (!whole) {
-      const uint32_t turned = p < r0 && from_v < r0 ? e4m3_rescale(was, ratio[1], ratio[1], ratio[1], ratio[1]) : was;
-      uint32_t mine = 0u, before = 0u;
+    for (int i = 0; i < VI; ++i) {
+      const int c = (tid + i * WRITE_THREADS) / hd;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        mine |= p + e >= r0 && p + e < r1 ? 0xffu << 8 * e : 0u;
-        before |= p + e < r0 ? 0xffu << 8 * e : 0u;
+      for (int j = 0; j < 4; ++j) {
+        const float4 x = make_float4(v[i][4 * j], v[i][4 * j + 1], v[i][4 * j + 2], v[i][4 * j + 3]);
+        const float m = wave_max(largest(x));
+        if (lane == 0) atomicMax(&top[hi][1][j], __float_as_uint(m));
+        if (!all_usable(x))
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int r = 16 * j + 4 * c + e;
+            if (!(fabsf(v[i][4 * j + e]) < E4M3_TOO_LARGE)) atomicOr(&bad[hi][r / 32], 1u << r % 32);
+          }
       }
-      w = (w & mine) | (turned & before) | (was & ~(mine | before));
     }
-    *at = w;
-  }
-  if (a.pages.weight) {
-    float* at = a.pages.weight + head * a.pages.page_size + in_page * E4M3_TILE;
-    if (tid >= r0 && tid < r1) at[tid] = 0.f;
+    __syncthreads();
+    const uint32_t bad0 = bad[hi][0], bad1 = bad[hi][1];
+    auto is_bad = [&](int r) { return ((r < 32 ? bad0 : bad1) >> (r % 32) & 1u) != 0u; };
+    if (bad0 | bad1) {      // once more without those rows (the same way for all threads)
+      __syncthreads();
+      if (tid < 8) top[hi][tid / 4][tid % 4] = 0u;
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < KI; ++i) {
+        const int r = (tid + i * WRITE_THREADS) / fours;
+        if (r < E4M3_TILE && !is_bad(r)) atomicMax(&top[hi][0][r / E4M3_BLOCK], __float_as_uint(largest(k[i])));
+      }
+#pragma unroll
+      for (int i = 0; i < VI; ++i) {
+        const int c = (tid + i * WRITE_THREADS) / hd;
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          if (c < 4 && !is_bad(16 * (j / 4) + 4 * c + j % 4)) atomicMax(&top[hi][1][j / 4], __float_as_uint(fabsf(v[i][j])));
+      }
+      __syncthreads();
+    }
+    if (tid < 8) {
+      const int m = tid / 4, j = tid % 4;
+      if (j * E4M3_BLOCK < r1 && (j + 1) * E4M3_BLOCK > r0) {
+        float* at = (m ? a.pages.v_scale : a.pages.k_scale) + e4m3_scale_at(a.pages, head, in_page) + j;
+        float scale = e4m3_scale(__uint_as_float(top[hi][m][j]));
+        if (j == r0 / E4M3_BLOCK) {
+          const float was = old0 < r0 ? *at : 0.f;
+          scale = fmaxf(scale, was);
+          ratio[hi % 2][m] = was * e4m3_inverse(scale);      // what the rows before the new ones are multiplied by (1: they stay)
+        }
+        *at = scale;
+        inverse[hi % 2][m][j] = e4m3_inverse(scale);
+      }
+    }
+    __syncthreads();
+    uint8_t* kt = a.pages.k + e4m3_tile_at(a.pages, head, in_page);
+    uint8_t* vt = a.pages.v + e4m3_tile_at(a.pages, head, in_page);
+    const float rk = ratio[hi % 2][0], rv = ratio[hi % 2][1];
+#pragma unroll
+    for (int i = 0; i < KI; ++i) {
+      const int at = tid + i * WRITE_THREADS, r = at / fours, d = at % fours * 4;
+      uint32_t* to = reinterpret_cast<uint32_t*>(kt + d / 16 * (16 * E4M3_TILE) + r * 16 + d % 16);
+      if (r >= r0 && r < r1) {
+        const float f = inverse[hi % 2][0][r / E4M3_BLOCK];
+        *to = is_bad(r) ? 0x7f7f7f7fu : e4m3_codes(k[i].x * f, k[i].y * f, k[i].z * f, k[i].w * f);
+      } else if (r >= old0 && r < r0 && rk != 1.f) {
+        *to = e4m3_rescale(*to, rk, rk, rk, rk);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < VI; ++i) {
+      const int at = tid + i * WRITE_THREADS, d = at % hd, c = at / hd;
+      if (c >= 4) break;
+      uint32_t* to = reinterpret_cast<uint32_t*>(vt + d * E4M3_TILE + 16 * c);
+      uint32_t w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float f = inverse[hi % 2][1][j];      // (of a block that is not written: whatever it is, its codes are not used)
+        float x[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = is_bad(16 * j + 4 * c + e) ? 0.f : v[i][4 * j + e] * f;
+        w[j] = e4m3_codes(x[0], x[1], x[2], x[3]);
+      }
+      if (r0 == 0 && r1 == E4M3_TILE) {
+        *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
+        continue;
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int p = 16 * j + 4 * c;
+        uint32_t mine = 0u, before = 0u;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          mine |= p + e >= r0 && p + e < r1 ? 0xffu << 8 * e : 0u;
+          before |= p + e >= old0 && p + e < r0 ? 0xffu << 8 * e : 0u;
+        }
+        if (rv == 1.f) before = 0u;
+        if (mine == 0xffffffffu) to[j] = w[j];
+        else if (mine | before) {
+          const uint32_t was = to[j], turned = before ? e4m3_rescale(was, rv, rv, rv, rv) : 0u;
+          to[j] = (w[j] & mine) | (turned & before) | (was & ~(mine | before));
+        }
+      }
+    }
+    if (a.pages.weight && tid >= r0 && tid < r1) a.pages.weight[head * a.pages.page_size + in_page * E4M3_TILE + tid] = 0.f;
   }
 }
 
@@ -216,25 +284,25 @@ TQ_API int tq_e4m3_write(const float* x, int64_t ld, const void* bias, int bias_
                          const int* table, int bt_stride, int page_size, int heads, int head0, hipStream_t st) {
   if (T <= 0 || B <= 0) return 0;
   if (rot < 0 || rot > hd || (rot & 1) || (pairing != 0 && pairing != 1) || (bias && bias_type != TQ_F32 && bias_type != TQ_BF16)) return TQ_ERR_BAD_ARG;
-  if (ld < (int64_t)(nh + 2 * nkv) * hd || ld % 4 != 0 || (uintptr_t)x % 16 != 0 || nh <= 0 || max_new <= 0) return TQ_ERR_BAD_ARG;
+  if (ld < (int64_t)(nh + 2 * nkv) * hd || ld % 4 != 0 || ld > (1 << 25) || (uintptr_t)x % 16 != 0 || nh <= 0 || max_new <= 0) return TQ_ERR_BAD_ARG;
   if (!e4m3_pages_fit(page_size, heads, head0, k ? nkv : 1, hd)) return TQ_ERR_UNSUPPORTED;
   E4m3Write a{x, ld, bias, bias_type, positions, inv_freq, pairing, rot, amp, cu, slots, start, (act_t*)q, T, B, nh, nkv, hd,
-              (max_new + E4M3_TILE - 2) / E4M3_TILE + 1, 1, nh,
+              (max_new + E4M3_TILE - 2) / E4M3_TILE + 1, 1, 1, nh,
               E4m3Pages{(uint8_t*)k, (uint8_t*)v, k_scale, v_scale, weight, table, bt_stride, page_size, heads, head0, hd}, k != nullptr};
-  // queries: as many tokens and heads to a workgroup as leave the chip a thousand of them
-  a.q_heads = nh;
-  while (a.q_heads > 1 && (int64_t)T * ((nh + a.q_heads - 1) / a.q_heads) < 1024) a.q_heads = (a.q_heads + 1) / 2;
-  while (a.q_tokens < 8 && (int64_t)T / a.q_tokens >= 4096) a.q_tokens *= 2;
-  const int64_t kv_groups = a.write ? (int64_t)a.tiles * nkv * B : 0;
+  // as many heads, and tokens of queries, to a workgroup (which share the angles) as leave the chip a few workgroups to a compute unit
+  while (a.write && a.kv_heads < WRITE_HEADS && a.kv_heads < nkv && (int64_t)a.tiles * B * nkv / a.kv_heads >= 1024) a.kv_heads *= 2;
+  while (a.q_heads > 1 && (int64_t)T * ((nh + a.q_heads - 1) / a.q_heads) < 512) a.q_heads = (a.q_heads + 1) / 2;
+  while (a.q_tokens < 8 && T / a.q_tokens >= 1024) a.q_tokens *= 2;
+  const int64_t kv_groups = a.write ? (int64_t)a.tiles * ((nkv + a.kv_heads - 1) / a.kv_heads) * B : 0;
   const int64_t groups = kv_groups + (int64_t)((T + a.q_tokens - 1) / a.q_tokens) * ((nh + a.q_heads - 1) / a.q_heads);
-  if (groups > 0xFFFFFF) return TQ_ERR_UNSUPPORTED;      // (a launch's threads are counted in 32 bits)
-  size_t shmem = (size_t)a.q_tokens * (rot / 2) * sizeof(float2);
-  if (a.write) shmem = max(shmem, 2 * (size_t)E4M3_TILE * (hd + 4) * sizeof(float));
-  if (shmem > 48 * 1024) {
-    const hipError_t e = hipFuncSetAttribute((const void*)e4m3_write_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)shmem);
-    if (e != hipSuccess) return (int)e;
-  }
-  hipLaunchKernelGGL(e4m3_write_kernel, dim3((unsigned)groups), dim3(256), shmem, st, a);
+  if (groups > 0x7FFFFF) return TQ_ERR_UNSUPPORTED;      // (a launch's threads are counted in 32 bits)
+  const size_t shmem = (size_t)(a.write ? min(E4M3_TILE, max(max_new, a.q_tokens)) : a.q_tokens) * (rot / 2) * sizeof(float2);      // at most 64 KiB
+  const dim3 grid((unsigned)groups), block(WRITE_THREADS);
+  const bool fours = rot % (pairing == 0 ? 8 : 4) == 0;
+  if (hd <= 128 && fours) hipLaunchKernelGGL((e4m3_write_kernel<4, true>), grid, block, shmem, st, a);
+  else if (hd <= 128) hipLaunchKernelGGL((e4m3_write_kernel<4, false>), grid, block, shmem, st, a);
+  else if (fours) hipLaunchKernelGGL((e4m3_write_kernel<8, true>), grid, block, shmem, st, a);
+  else hipLaunchKernelGGL((e4m3_write_kernel<8, false>), grid, block, shmem, st, a);
   TQ_LAUNCH_CHECK();
   return 0;
 }

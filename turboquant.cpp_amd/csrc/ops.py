@@ -171,7 +171,7 @@ _SIGNATURES = {
                        _c_ptr],
     "tq_e4m3_move": [_c_ptr, _c_ptr, _c_int, _c_ptr, _c_int, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int,
                      _c_int, _c_int, _c_ptr],
-    "tq_e4m3_attention_scratch": [_c_int] * 7,
+    "tq_e4m3_attention_scratch": [_c_int] * 8,
     "tq_e4m3_attention": [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_f32, _c_f32, _c_ptr,
                           _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_ptr,
                           _c_int, _c_int, _c_int, _c_ptr],
@@ -1348,7 +1348,7 @@ def attention_writes_into(act, head_dim: int, scale: float) -> bool:
 E4M3_BLOCK = 16      # positions that share a scale
 
 
-@dataclasses.dataclass
+@dataclasses.dataclass(frozen=True, eq=False)
 class E4m3Pages:
     """Pages of keys and values as e4m3 codes with a scale, a power of two, for each block of 16 positions of a layer's kv head.
 
@@ -1370,6 +1370,33 @@ class E4m3Pages:
     table: torch.Tensor
     weight: torch.Tensor | None = None
 
+    def __post_init__(self):
+        """Checks the pools once, for all calls with these pages."""
+        k, dev = "E4m3Pages", self.k.get_device()
+        shape = self.k.shape
+        _need(len(shape) == 4 and dev >= 0, k, "k must be [pages, layers, kv heads, page_size * head_dim] on the GPU")
+        ps = self.k_scale.shape[-1] * E4M3_BLOCK
+        _need(ps > 0 and ps % 64 == 0, k, lambda: f"pages must hold a multiple of 64 positions, hold {ps}")
+        _need(shape[3] % (16 * ps) == 0 and 16 <= shape[3] // ps <= 256, k,
+              lambda: f"a head of {shape[3] / ps:g} numbers is none of the multiples of 16 up to 256 that 8-bit pages take")
+        pools = [("k", self.k, torch.float8_e4m3fn, shape), ("v", self.v, torch.float8_e4m3fn, shape),
+                 ("k_scale", self.k_scale, torch.float32, (*shape[:3], ps // E4M3_BLOCK)),
+                 ("v_scale", self.v_scale, torch.float32, (*shape[:3], ps // E4M3_BLOCK))]
+        if self.weight is not None:
+            pools.append(("weight", self.weight, torch.float32, (*shape[:3], ps)))
+        for name, t, dtype, want in pools:
+            _check_here(t, k, name, dtype, want, dev)
+        _check_here(self.table, k, "table", torch.int32, None, dev)
+        _need(self.table.dim() == 2, k, "table must be [slots, pages]")
+        _need(min(shape[:3]) >= 1 and self.k.data_ptr() % 16 == 0 and self.v.data_ptr() % 16 == 0, k, "pools must hold pages, from a multiple of 16 bytes on")
+        put = object.__setattr__
+        put(self, "page_size", ps)
+        put(self, "head_dim", shape[3] // ps)
+        put(self, "layers", shape[1])
+        put(self, "num_kv_heads", shape[2])
+        put(self, "device_index", dev)
+        put(self, "table_shape", tuple(self.table.shape))
+
     @classmethod
     def empty(cls, n_pages: int, layers: int, num_kv_heads: int, head_dim: int, page_size: int, table: torch.Tensor,
               weights: bool = False) -> "E4m3Pages":
@@ -1380,46 +1407,36 @@ class E4m3Pages:
         scale = [torch.zeros((*rows, page_size // E4M3_BLOCK), dtype=torch.float32, device=dev) for _ in range(2)]
         return cls(*pool, *scale, table, torch.zeros((*rows, page_size), dtype=torch.float32, device=dev) if weights else None)
 
-    @property
-    def page_size(self) -> int:
-        return self.k_scale.shape[-1] * E4M3_BLOCK
+    def _args(self, layer: int, weight: bool) -> tuple:
+        return (self.k.data_ptr(), self.v.data_ptr(), self.k_scale.data_ptr(), self.v_scale.data_ptr(),
+                self.weight.data_ptr() if weight and self.weight is not None else None, self.table.data_ptr(), self.table_shape[1],
+                self.page_size, self.layers * self.num_kv_heads, layer * self.num_kv_heads)
 
-    @property
-    def head_dim(self) -> int:
-        return self.k.shape[-1] // self.page_size
-
-    def check(self, k: str, device, layer: int = 0) -> None:
-        for name, t, dtype in (("k", self.k, torch.float8_e4m3fn), ("v", self.v, torch.float8_e4m3fn), ("k_scale", self.k_scale, torch.float32),
-                               ("v_scale", self.v_scale, torch.float32), ("weight", self.weight, torch.float32)):
-            if t is not None:
-                _check(t, k, name, dtype)
-                _need(t.dim() == 4 and t.shape[:3] == self.k.shape[:3] and t.device == device, k,
-                      lambda: f"{name} must be [pages, layers, kv heads, ...] as the other pools are, on the same GPU, is {tuple(t.shape)}")
-        _check(self.table, k, "table", torch.int32)
-        _need(self.table.dim() == 2 and self.table.device == device, k, "table must be [slots, pages] on the same GPU")
-        ps = self.page_size
-        _need(ps > 0 and ps % 64 == 0, k, lambda: f"pages must hold a multiple of 64 positions, hold {ps}")
-        _need(self.k.shape[3] % ps == 0 and self.v.shape == self.k.shape and self.v_scale.shape == self.k_scale.shape, k,
-              "pools of keys and values must have one shape, page_size * head_dim numbers to a page's head")
-        _need(self.head_dim % 16 == 0 and 16 <= self.head_dim <= 256, k,
-              lambda: f"head size {self.head_dim} is none of the multiples of 16 up to 256 that 8-bit pages take")
-        _need(self.weight is None or self.weight.shape[3] == ps, k, "weight must have a number for every position")
-        _need(0 <= layer < self.k.shape[1], k, lambda: f"layer {layer} is none of the pages' {self.k.shape[1]}")
+    def _here(self, k: str, layer: int = 0) -> int:
+        """The pages' device, which has to be the current one; whether they have that layer."""
+        _need(self.device_index == torch.cuda.current_device(), k, lambda: f"the pages lie on GPU {self.device_index}, which is not the current device")
+        _need(0 <= layer < self.layers, k, lambda: f"layer {layer} is none of the pages' {self.layers}")
+        return self.device_index
 
 
-def _e4m3_runs(k: str, runs: dict, pages: E4m3Pages, T: int, device) -> int:
-    B = runs["slots"].numel()
-    _check(runs["cu_seqlens"], k, "cu_seqlens", torch.int32, (B + 1,))
-    _check(runs["slots"], k, "slots", torch.int32, (B,))
-    _check(runs["start"], k, "start", torch.int32, (B,))
-    _need(all(runs[n].device == device for n in ("cu_seqlens", "slots", "start")), k, "the runs must lie on the same GPU")
-    _need(0 < int(runs["max_end"]) <= pages.table.shape[1] * pages.page_size, k, "positions reach beyond the page table")
-    _need(1 <= int(runs["max_new"]) <= T and (not runs["decode"] or T == B), k, "decoding brings one token per sequence")
-    return B
+def _check_here(t: torch.Tensor, kernel: str, name: str, dtype, shape, device: int) -> None:
+    """``_check`` and that the tensor lies on GPU ``device``, in as little of the host's time as a call that is right needs."""
+    if not (isinstance(t, torch.Tensor) and t.dtype is dtype and (shape is None or t.shape == shape) and t.get_device() == device and t.is_contiguous()):
+        _check(t, kernel, name, dtype, shape)
+        raise KernelError(f"{kernel}: {name} lies on {t.device}, the other tensors on GPU {device}")
 
 
-def _same_device(k: str, device) -> None:
-    _need(device.index == torch.cuda.current_device(), k, lambda: f"the tensors lie on {device}, which is not the current device")
+def _e4m3_runs(k: str, runs: dict, pages: E4m3Pages, T: int, dev: int):
+    cu, slots, start = runs["cu_seqlens"], runs["slots"], runs["start"]
+    B = slots.numel()
+    _check_here(cu, k, "cu_seqlens", torch.int32, (B + 1,), dev)
+    _check_here(slots, k, "slots", torch.int32, (B,), dev)
+    _check_here(start, k, "start", torch.int32, (B,), dev)
+    max_new, max_end, decode = int(runs["max_new"]), int(runs["max_end"]), bool(runs["decode"])
+    _need(0 < max_end <= pages.table_shape[1] * pages.page_size, k, "positions reach beyond the page table")
+    _need(1 <= max_new <= T and B <= T, k, "the runs do not fit the tokens")
+    _need(not decode or (T == B and max_new == 1), k, "decoding brings one token per sequence")
+    return (cu.data_ptr(), slots.data_ptr(), start.data_ptr()), B, max_new, max_end, decode
 
 
 def rope_kv_write_e4m3(qkv: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, pairing: int, rotary_dim: int,
@@ -1432,30 +1449,32 @@ def rope_kv_write_e4m3(qkv: torch.Tensor, positions: torch.Tensor, inv_freq: tor
     start at zero.  ``write`` False: the queries alone, for a layer that reads another layer's cache (``qkv`` then holds no keys
     and values)."""
     k = "rope_kv_write_e4m3"
-    T = positions.numel()
-    _check(positions, k, "positions", torch.int32, (T,))
-    pages.check(k, positions.device, layer)
-    _same_device(k, positions.device)
-    nkv, hd = pages.k.shape[2], pages.head_dim
-    width = (num_heads + (2 * nkv if write else 0)) * hd
+    dev, T = pages._here(k, layer), positions.numel()
+    nkv, hd = pages.num_kv_heads if write else 0, pages.head_dim
+    width = (num_heads + 2 * nkv) * hd
     _need(num_heads >= 1 and T >= 1, k, "there must be a head and a token")
-    _need(isinstance(qkv, torch.Tensor) and qkv.device == positions.device and qkv.dtype == torch.float32 and tuple(qkv.shape) == (T, width)
-          and qkv.stride(1) == 1 and (qkv.stride(0) >= width or T == 1), k,
-          lambda: f"qkv must be float32 [{T}, {width}] on the GPU with unit stride along its rows")
-    _need((T == 1 or qkv.stride(0) % 4 == 0) and qkv.data_ptr() % 16 == 0, k, "rows of qkv must start at multiples of 16 bytes")
+    _check_here(positions, k, "positions", torch.int32, (T,), dev)
+    _need(isinstance(qkv, torch.Tensor) and qkv.get_device() == dev and qkv.dtype is torch.float32 and qkv.shape == (T, width), k,
+          lambda: f"qkv must be float32 [{T}, {width}] on GPU {dev}")
+    ld, one = qkv.stride()
+    if T == 1:
+        ld = width
+    _need(one == 1 and ld >= width and ld % 4 == 0 and qkv.data_ptr() % 16 == 0, k,
+          "rows of qkv must have unit stride and start at multiples of 16 bytes")
     if bias is not None:
-        _check(bias, k, "bias", tuple(_WTYPE), (width,))
-    _check(inv_freq, k, "inv_freq", torch.float32)
-    _need(0 <= rotary_dim <= hd and rotary_dim % 2 == 0 and pairing in (0, 1) and (rotary_dim == 0 or inv_freq.numel() * 2 == rotary_dim), k,
-          lambda: f"inv_freq must hold rotary_dim/2 = {rotary_dim // 2} entries, for at most a head's {hd} numbers")
-    B = _e4m3_runs(k, runs, pages, T, positions.device)
-    q = torch.empty((T, num_heads * hd), dtype=ACT_DTYPES[dtype_name(act)], device=positions.device)
-    ld = qkv.stride(0) if T > 1 else width
+        _check_here(bias, k, "bias", torch.bfloat16 if bias.dtype is torch.bfloat16 else torch.float32, (width,), dev)
+    _need(0 <= rotary_dim <= hd and rotary_dim % 2 == 0 and (pairing == 0 or pairing == 1), k,
+          lambda: f"rotary_dim must be even and at most a head's {hd}, pairing 0 or 1")
+    _check_here(inv_freq, k, "inv_freq", torch.float32, (rotary_dim // 2,) if rotary_dim else None, dev)
+    where, B, max_new, _max_end, _decode = _e4m3_runs(k, runs, pages, T, dev)
+    act = dtype_name(act)
+    q = torch.empty((T, num_heads * hd), dtype=ACT_DTYPES[act], device=positions.device)
+    pools = pages._args(layer, True)
+    if not write:
+        pools = (None, *pools[1:])
     _run(k, library(act).tq_e4m3_write(
-        _ptr(qkv), ld, _ptr(bias), _WTYPE[bias.dtype] if bias is not None else 0, _ptr(positions), _ptr(inv_freq), pairing, rotary_dim,
-        float(amplitude), _ptr(runs["cu_seqlens"]), _ptr(runs["slots"]), _ptr(runs["start"]), _ptr(q), T, B, int(runs["max_new"]), num_heads,
-        nkv if write else 0, hd, _ptr(pages.k) if write else None, _ptr(pages.v) if write else None, _ptr(pages.k_scale), _ptr(pages.v_scale),
-        _ptr(pages.weight), _ptr(pages.table), pages.table.shape[1], pages.page_size, pages.k.shape[1] * nkv, layer * nkv, _stream()))
+        qkv.data_ptr(), ld, _ptr(bias), 0 if bias is None else _WTYPE[bias.dtype], positions.data_ptr(), inv_freq.data_ptr(), pairing, rotary_dim,
+        amplitude, *where, q.data_ptr(), T, B, max_new, num_heads, nkv, hd, *pools, _raw_stream(dev)))
     return q
 
 
@@ -1468,36 +1487,40 @@ def attention_e4m3(q: torch.Tensor, pages: E4m3Pages, layer: int, num_heads: int
     exp(score) over the softmax's denominator (sums in a fixed order: the same step gives the same bits).  A row whose scores are
     all -inf is 0 and gives no weight."""
     k = "attention_e4m3"
-    adt = ACT_DTYPES[dtype_name(act)]
-    _need(isinstance(q, torch.Tensor) and q.is_cuda and q.dim() == 2, k, "q must be [T, heads * head_dim] on the GPU")
-    pages.check(k, q.device, layer)
-    _same_device(k, q.device)
-    T, nkv, hd = q.shape[0], pages.k.shape[2], pages.head_dim
-    _check(q, k, "q", adt, (T, num_heads * hd))
+    dev, act = pages._here(k, layer), dtype_name(act)
+    _need(isinstance(q, torch.Tensor) and q.dim() == 2, k, "q must be [T, heads * head_dim]")
+    T, nkv, hd = q.shape[0], pages.num_kv_heads, pages.head_dim
+    _need(T >= 1 and num_heads >= 1 and num_heads % nkv == 0, k, "heads must be a multiple of kv heads, and there must be a token")
+    _check_here(q, k, "q", ACT_DTYPES[act], (T, num_heads * hd), dev)
     _need(q.data_ptr() % 16 == 0, k, "q must start at a multiple of 16 bytes")
-    _need(num_heads >= 1 and num_heads % nkv == 0, k, "heads must be a multiple of kv heads")
     _need(math.isfinite(scale), k, "scale must be finite")
-    _need((window is None or window >= 1) and (chunk is None or chunk >= 1) and (softcap is None or softcap > 0), k,
+    _need((window is None or window >= 1) and (chunk is None or chunk >= 1) and (softcap is None or 0 < softcap < math.inf), k,
           "window, chunk and softcap must be positive")
     r1 = r2 = None
     if distance_bias is not None:
         r1, r2 = distance_bias
-        _check(r1, k, "r1", torch.float32, (num_heads,))
-        _check(r2, k, "r2", torch.float32, (num_heads,))
+        _check_here(r1, k, "r1", torch.float32, (num_heads,), dev)
+        _check_here(r2, k, "r2", torch.float32, (num_heads,), dev)
     if sink is not None:
-        _check(sink, k, "sink", torch.float32, (num_heads,))
+        _check_here(sink, k, "sink", torch.float32, (num_heads,), dev)
     _need(not add_weights or pages.weight is not None, k, "these pages keep no weights")
-    B = _e4m3_runs(k, runs, pages, T, q.device)
-    lib, decode = library(act), int(bool(runs["decode"]))
+    where, B, max_new, max_end, decode = _e4m3_runs(k, runs, pages, T, dev)
+    lib = library(act)
     out = torch.empty_like(q)
-    n = lib.tq_e4m3_attention_scratch(T, B, num_heads, hd, int(runs["max_end"]), decode, int(add_weights))
+    n = lib.tq_e4m3_attention_scratch(T, B, num_heads, nkv, hd, max_end, decode, add_weights) if decode or add_weights else 0
     scratch = torch.empty((n,), dtype=torch.float32, device=q.device) if n else None
     _run(k, lib.tq_e4m3_attention(
-        _ptr(q), _ptr(out), _ptr(runs["cu_seqlens"]), _ptr(runs["slots"]), _ptr(runs["start"]), T, B, num_heads, nkv, hd, int(window or 0),
-        float(scale), float(softcap or 0.0), _ptr(r1), _ptr(r2), int(chunk or 0), _ptr(sink), _ptr(pages.k), _ptr(pages.v),
-        _ptr(pages.k_scale), _ptr(pages.v_scale), _ptr(pages.weight) if add_weights else None, _ptr(pages.table), pages.table.shape[1],
-        pages.page_size, pages.k.shape[1] * nkv, layer * nkv, _ptr(scratch), decode, int(runs["max_new"]), int(runs["max_end"]), _stream()))
+        q.data_ptr(), out.data_ptr(), *where, T, B, num_heads, nkv, hd, window or 0, scale, softcap or 0.0, _ptr(r1), _ptr(r2), chunk or 0,
+        _ptr(sink), *pages._args(layer, add_weights), _ptr(scratch), decode, max_new, max_end, _raw_stream(dev)))
     return out
+
+
+def _evict_slots(k: str, pages: E4m3Pages, slots: torch.Tensor, name: str) -> tuple[int, int]:
+    dev = pages._here(k)
+    _need(isinstance(slots, torch.Tensor) and slots.dim() == 1, k, lambda: f"{name} must be [B]")
+    B = slots.numel()
+    _check_here(slots, k, name, torch.int32, (B,), dev)
+    return dev, B
 
 
 def evict_choose(pages: E4m3Pages, slots: torch.Tensor, lengths: torch.Tensor, max_length: int, keep: int, first: int = 0,
@@ -1507,22 +1530,16 @@ def evict_choose(pages: E4m3Pages, slots: torch.Tensor, lengths: torch.Tensor, m
     in all; of equal weights the lower position stays, and NaN counts as the largest.  int32 [B, layers, kv heads, keep] in ascending
     order.  A sequence of ``keep`` positions or fewer keeps them all, with -1 behind them."""
     k = "evict_choose"
-    _need(isinstance(slots, torch.Tensor) and slots.is_cuda and slots.dim() == 1, k, "slots must be [B] on the GPU")
-    B = slots.numel()
-    _check(slots, k, "slots", torch.int32, (B,))
-    _check(lengths, k, "lengths", torch.int32, (B,))
-    pages.check(k, slots.device)
-    _same_device(k, slots.device)
-    _need(lengths.device == slots.device, k, "lengths must lie on the same GPU")
+    dev, B = _evict_slots(k, pages, slots, "slots")
+    _check_here(lengths, k, "lengths", torch.int32, (B,), dev)
     _need(pages.weight is not None, k, "these pages keep no weights")
     _need(keep >= 1 and first >= 0 and recent >= 0 and first + recent <= keep, k,
           lambda: f"the first {first} and last {recent} positions must lie within the {keep} that stay")
-    _need(0 <= max_length <= pages.table.shape[1] * pages.page_size, k, "positions reach beyond the page table")
-    layers, nkv = pages.k.shape[1:3]
-    kept = torch.empty((B, layers, nkv, keep), dtype=torch.int32, device=slots.device)
-    _run(k, library(act).tq_e4m3_choose(_ptr(slots), _ptr(lengths), B, int(max_length), int(keep), int(first), int(recent), _ptr(kept),
-                                        _ptr(pages.weight), _ptr(pages.table), pages.table.shape[0], pages.table.shape[1],
-                                        pages.page_size, layers * nkv, _stream()))
+    _need(0 <= max_length <= pages.table_shape[1] * pages.page_size, k, "positions reach beyond the page table")
+    kept = torch.empty((B, pages.layers, pages.num_kv_heads, keep), dtype=torch.int32, device=slots.device)
+    _run(k, library(act).tq_e4m3_choose(slots.data_ptr(), lengths.data_ptr(), B, max_length, keep, first, recent, kept.data_ptr(),
+                                        pages.weight.data_ptr(), pages.table.data_ptr(), *pages.table_shape, pages.page_size,
+                                        pages.layers * pages.num_kv_heads, _raw_stream(dev)))
     return kept
 
 
@@ -1532,21 +1549,15 @@ def evict_move(pages: E4m3Pages, src_slots: torch.Tensor, dst_slots: torch.Tenso
     is copied in place.  A block's scale becomes the largest of its rows'; what lies behind the last row in its page becomes zero.  A
     row of the table that is -1 where a page is written, or a slot outside the table, is passed over."""
     k = "evict_move"
-    _need(isinstance(src_slots, torch.Tensor) and src_slots.is_cuda and src_slots.dim() == 1, k, "src_slots must be [B] on the GPU")
-    B = src_slots.numel()
-    _check(src_slots, k, "src_slots", torch.int32, (B,))
-    _check(dst_slots, k, "dst_slots", torch.int32, (B,))
-    pages.check(k, src_slots.device)
-    _same_device(k, src_slots.device)
-    layers, nkv = pages.k.shape[1:3]
-    _check(kept, k, "kept", torch.int32)
-    _need(kept.dim() == 4 and tuple(kept.shape[:3]) == (B, layers, nkv) and kept.shape[3] >= 1, k,
-          lambda: f"kept must be [{B}, {layers}, {nkv}, keep]")
-    _need(dst_slots.device == src_slots.device and kept.device == src_slots.device, k, "dst_slots and kept must lie on the same GPU")
-    _need(kept.shape[3] <= pages.table.shape[1] * pages.page_size, k, "positions reach beyond the page table")
-    _run(k, library(act).tq_e4m3_move(_ptr(src_slots), _ptr(dst_slots), B, _ptr(kept), kept.shape[3], pages.head_dim, _ptr(pages.k),
-                                      _ptr(pages.v), _ptr(pages.k_scale), _ptr(pages.v_scale), _ptr(pages.weight), _ptr(pages.table),
-                                      pages.table.shape[0], pages.table.shape[1], pages.page_size, layers * nkv, _stream()))
+    dev, B = _evict_slots(k, pages, src_slots, "src_slots")
+    _check_here(dst_slots, k, "dst_slots", torch.int32, (B,), dev)
+    _need(isinstance(kept, torch.Tensor) and kept.dim() == 4 and kept.shape[3] >= 1, k, "kept must be [B, layers, kv heads, keep]")
+    keep = kept.shape[3]
+    _check_here(kept, k, "kept", torch.int32, (B, pages.layers, pages.num_kv_heads, keep), dev)
+    _need(keep <= pages.table_shape[1] * pages.page_size, k, "positions reach beyond the page table")
+    pools = pages._args(0, True)
+    _run(k, library(act).tq_e4m3_move(src_slots.data_ptr(), dst_slots.data_ptr(), B, kept.data_ptr(), keep, pages.head_dim, *pools[:6],
+                                      *pages.table_shape, *pools[7:9], _raw_stream(dev)))
 
 
 # ------------------------------------------------------------------ routing
