@@ -298,43 +298,77 @@ struct DecodeWave {
   }
 };
 
-// One wave joins the runs [beg, end) of one head, `stride` numbers apart, and writes the output row; gives log2 of the row's sum.
-// Denominators are added 64 runs at a time, sums in four strands by run, which are added at the end.  `mine`: the strand of a wave
-// that shares the head with three others (their strands meet in `strands`, [4][256]), or -1: all four.
-template <int MINE>
-__device__ __forceinline__ float join_runs(const E4m3Attn& a, const float* part, int stride, int beg, int end, int h, int64_t t, int mine, float* strands) {
+// The maximum of a head's runs [beg, end), `stride` numbers apart, and the sink; and the sum of their denominators brought to it, 64
+// runs at a time.  `w`: of the first 64 runs, the lane's run's factor.
+__device__ __forceinline__ void join_sums(const E4m3Attn& a, const float* part, int stride, int beg, int end, int h, float& m, float& l, float& w) {
   const int lane = threadIdx.x % 64, hd = a.pages.hd;
-  float m = a.mod.sink ? a.mod.sink[h] * LOG2E : -INFINITY;
-  for (int i = beg + lane; i < end; i += 64) m = fmaxf(m, part[(int64_t)i * stride + hd]);
+  // (the first 64 runs' two numbers at once: most sequences have no more)
+  const float* mine = part + (int64_t)min(beg + lane, end - 1) * stride + hd;
+  const float m0 = mine[0], l0 = mine[1];
+  m = fmaxf(a.mod.sink ? a.mod.sink[h] * LOG2E : -INFINITY, beg + lane < end ? m0 : -INFINITY);
+  for (int i = beg + 64 + lane; i < end; i += 64) m = fmaxf(m, part[(int64_t)i * stride + hd]);
   m = wave_max(m);
   const float use = m == -INFINITY ? 0.f : m;
-  float l = a.mod.sink ? __builtin_amdgcn_exp2f(a.mod.sink[h] * LOG2E - use) : 0.f;
-  float acc[MINE == 0 ? 4 : 1][4] = {};
-  for (int i0 = beg; i0 < end; i0 += 64) {
+  l = a.mod.sink ? __builtin_amdgcn_exp2f(a.mod.sink[h] * LOG2E - use) : 0.f;
+  w = beg + lane < end ? __builtin_amdgcn_exp2f(m0 - use) : 0.f;
+  l += wave_sum(beg + lane < end ? w * l0 : 0.f);
+  for (int i0 = beg + 64; i0 < end; i0 += 64) {
     const int i = i0 + lane;
-    float w = 0.f, wl = 0.f;
-    if (i < end) {
-      w = __builtin_amdgcn_exp2f(part[(int64_t)i * stride + hd] - use);
-      wl = w * part[(int64_t)i * stride + hd + 1];
+    l += wave_sum(i < end ? __builtin_amdgcn_exp2f(part[(int64_t)i * stride + hd] - use) * part[(int64_t)i * stride + hd + 1] : 0.f);
+  }
+}
+// Joins the runs of one head and writes the output row; gives log2 of the row's sum.  Values are added in four strands by run, and the
+// strands at the end.  MINE: the wave shares the head with three others and takes strand `mine` (the strands meet in `strands`,
+// [4][256]); else it takes all four.
+template <bool MINE>
+__device__ __forceinline__ float join_runs(const E4m3Attn& a, const float* part, int stride, int beg, int end, int h, int64_t t, int mine, float* strands) {
+  constexpr int NS = MINE ? 1 : 4, NJ = MINE ? 16 : 1;
+  const int lane = threadIdx.x % 64, hd = a.pages.hd;
+  float v[NJ][4] = {};
+  // a strand's values of 64 runs are asked for before the factors are known
+  auto ask = [&](int i0) {
+#pragma unroll
+    for (int k = 0; k < NJ; ++k)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (64 * e < hd && i0 + 4 * k + mine < end) v[k][e] = part[(int64_t)(i0 + 4 * k + mine) * stride + min(64 * e + lane, hd - 1)];
+  };
+  if constexpr (MINE) ask(beg);
+  float m, l, w;
+  join_sums(a, part, stride, beg, end, h, m, l, w);
+  const float use = m == -INFINITY ? 0.f : m;
+  float acc[NS][4] = {};
+  for (int i0 = beg; i0 < end; i0 += 64) {
+    if (i0 > beg) {
+      w = i0 + lane < end ? __builtin_amdgcn_exp2f(part[(int64_t)(i0 + lane) * stride + hd] - use) : 0.f;
+      if constexpr (MINE) ask(i0);
     }
-    l += wave_sum(wl);
     const int n = min(64, end - i0);
-#pragma unroll(MINE == 0 ? 2 : 8)
-    for (int j = MINE == 0 ? 0 : mine; j < n; j += 4) {
+    if constexpr (MINE) {
 #pragma unroll
-      for (int s = 0; s < (MINE == 0 ? 4 : 1); ++s) {
-        if (j + s >= n) break;
-        const float ws = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), j + s));
-        const float* from = part + (int64_t)(i0 + j + s) * stride;
+      for (int k = 0; k < NJ; ++k) {
+        if (4 * k + mine >= n) break;
+        const float ws = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), 4 * k + mine));
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (64 * e < hd) acc[s][e] = fmaf(ws, from[min(64 * e + lane, hd - 1)], acc[s][e]);
+        for (int e = 0; e < 4; ++e) acc[0][e] = fmaf(ws, v[k][e], acc[0][e]);
+      }
+    } else {
+#pragma unroll 2
+      for (int j = 0; j < n; j += 4) {
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+          if (j + s >= n) break;
+          const float ws = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), j + s));
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (64 * e < hd) acc[s][e] = fmaf(ws, part[(int64_t)(i0 + j + s) * stride + min(64 * e + lane, hd - 1)], acc[s][e]);
+        }
       }
     }
   }
   const float inv = over(l);
   act_t* out = a.out + (t * a.nh + h) * hd;
-  if constexpr (MINE != 0) {
+  if constexpr (MINE) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) strands[256 * mine + 64 * e + lane] = acc[0][e];
     __syncthreads();
@@ -347,31 +381,32 @@ __device__ __forceinline__ float join_runs(const E4m3Attn& a, const float* part,
   }
   return lse_of(m, l);
 }
-// log2 of a row's sum alone, as join_runs gives it.
-__device__ __forceinline__ float lse_of_runs(const E4m3Attn& a, const float* part, int stride, int beg, int end, int h) {
-  const int lane = threadIdx.x % 64, hd = a.pages.hd;
-  float m = a.mod.sink ? a.mod.sink[h] * LOG2E : -INFINITY;
-  for (int i = beg + lane; i < end; i += 64) m = fmaxf(m, part[(int64_t)i * stride + hd]);
-  m = wave_max(m);
-  const float use = m == -INFINITY ? 0.f : m;
-  float l = a.mod.sink ? __builtin_amdgcn_exp2f(a.mod.sink[h] * LOG2E - use) : 0.f;
-  for (int i0 = beg; i0 < end; i0 += 64) {
-    const int i = i0 + lane;
-    l += wave_sum(i < end ? __builtin_amdgcn_exp2f(part[(int64_t)i * stride + hd] - use) * part[(int64_t)i * stride + hd + 1] : 0.f);
+// A position's weight of one token: the sum over the g heads of a kv head, whose sums `lse` has.  `ask` first, for eight heads' scores.
+struct WeightOf {
+  float s[8];
+  __device__ __forceinline__ void ask(const E4m3Attn& a, int b, int kvh, int i0, int j) {
+    const int g = a.nh / a.nkv;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i0 + i < g) s[i] = a.scores[((int64_t)b * a.nh + kvh * g + i0 + i) * a.ld_scores + j];
   }
-  return lse_of(m, l);
-}
-// A position's weight of one token: the sum over the g heads of a kv head, whose sums `lse` has.
-__device__ __forceinline__ void add_weight(const E4m3Attn& a, const int* row, int b, int kvh, int j, const float* lse) {
-  const int g = a.nh / a.nkv;
-  int in_page;
-  const int64_t head = e4m3_head_of(a.pages, row, j / E4M3_TILE, kvh, in_page);
-  if (head < 0) return;
-  float w = 0.f;
-  for (int i = 0; i < g; ++i)
-    w += __builtin_amdgcn_exp2f(a.scores[((int64_t)b * a.nh + kvh * g + i) * a.ld_scores + j] - lse[i]);
-  a.pages.weight[head * a.pages.page_size + in_page * E4M3_TILE + j % E4M3_TILE] += w;
-}
+  __device__ __forceinline__ void add(const E4m3Attn& a, const int* row, int b, int kvh, int j, const float* lse) {
+    const int g = a.nh / a.nkv;
+    int in_page;
+    const int64_t head = e4m3_head_of(a.pages, row, j / E4M3_TILE, kvh, in_page);
+    if (head < 0) return;
+    float* to = a.pages.weight + head * a.pages.page_size + in_page * E4M3_TILE + j % E4M3_TILE;
+    const float was = *to;
+    float w = 0.f;
+    for (int i0 = 0; i0 < g; i0 += 8) {
+      if (i0) ask(a, b, kvh, i0, j);
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (i0 + i < g) w += __builtin_amdgcn_exp2f(s[i] - lse[i0 + i]);
+    }
+    *to = was + w;
+  }
+};
 
 // Runs of all but the shortest sequences: grid (waves, nkv * ceil(g / 16), B), block 64; a wave streams through neighbouring runs.
 template <int DT, bool MOD>
@@ -404,19 +439,24 @@ __global__ __launch_bounds__(256) void e4m3_join_kernel(E4m3Attn a, int blocks_o
   const int beg = lo / E4M3_TILE / S, end = p / E4M3_TILE / S + 1;
   if (joins) {
     const int h = x % a.nh;
-    join_runs<1>(a, a.partial + ((int64_t)b * a.nh + h) * a.max_runs * stride, stride, beg, end, h, a.cu[b], wave, lds);
+    join_runs<true>(a, a.partial + ((int64_t)b * a.nh + h) * a.max_runs * stride, stride, beg, end, h, a.cu[b], wave, lds);
     return;
   }
   const int kvh = x / blocks_of_weights % a.nkv, j = x % blocks_of_weights * 256 + (int)threadIdx.x;
   if (j - (int)threadIdx.x > p || j - (int)threadIdx.x + 255 < lo) return;
   const int* row = a.pages.table + (int64_t)a.slots[b] * a.pages.bt_stride;
+  const bool has = j >= lo && j <= p;
+  WeightOf of;
+  if (has) of.ask(a, b, kvh, 0, j);
+#pragma unroll 2
   for (int i = wave; i < g; i += 4) {      // (at most 1,024 heads to a kv head: the launcher has checked)
     const int h = kvh * g + i;
-    const float lse = lse_of_runs(a, a.partial + ((int64_t)b * a.nh + h) * a.max_runs * stride, stride, beg, end, h);
-    if (lane == 0) lds[i] = lse;
+    float m, l, w;
+    join_sums(a, a.partial + ((int64_t)b * a.nh + h) * a.max_runs * stride, stride, beg, end, h, m, l, w);
+    if (lane == 0) lds[i] = lse_of(m, l);
   }
   __syncthreads();
-  if (j >= lo && j <= p) add_weight(a, row, b, kvh, j, lds);
+  if (has) of.add(a, row, b, kvh, j, lds);
 }
 
 // A step whose sequences all hold at most SHORT_END positions: grid (nkv * ceil(g / 16), B), one launch.
@@ -438,13 +478,17 @@ __global__ __launch_bounds__(64 * SHORT_WAVES) __attribute__((amdgpu_waves_per_e
   }
   __syncthreads();
   for (int i = wave; i < heads; i += SHORT_WAVES) {
-    const float x = join_runs<0>(a, sums + i * stride, heads * stride, 0, end - beg, kvh * g + 16 * cg + i, a.cu[b], -1, nullptr);
+    const float x = join_runs<false>(a, sums + i * stride, heads * stride, 0, end - beg, kvh * g + 16 * cg + i, a.cu[b], -1, nullptr);
     if (lane == 0) lse[i] = x;
   }
   if (!a.scores) return;
   __threadfence_block();      // (the scores that the workgroup's waves have written)
   __syncthreads();
-  for (int j = max(w.lo, beg * E4M3_TILE) + (int)threadIdx.x; j <= w.p; j += 64 * SHORT_WAVES) add_weight(a, w.row, b, kvh, j, lse);
+  for (int j = max(w.lo, beg * E4M3_TILE) + (int)threadIdx.x; j <= w.p; j += 64 * SHORT_WAVES) {
+    WeightOf of;
+    of.ask(a, b, kvh, 0, j);
+    of.add(a, w.row, b, kvh, j, lse);
+  }
 }
 
 // ------------------------------------------------------------------------------------------ prompts
@@ -688,7 +732,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DT > 8 ? 1 
 }
 
 // ------------------------------------------------------------------------------------------ launch
-#define DECODE_WAVES 4096      // waves of a step beyond which a wave takes more runs instead
+// Waves of a step beyond which a wave takes more runs instead: two rounds of three waves to a SIMD.  us of the runs of 8 sequences of 8,192 tokens (16
+// heads) and of 64 of 300 to 4,100 (28 heads on 4): with 2,048 waves 52 and 55, 3,072 53 and 51, 4,096 59 and 51, 6,144 52 and 42, 8,192 55 and 42.
+#define DECODE_WAVES 6144
 template <int DT, bool MOD>
 static int launch_decode(const E4m3Attn& a, int max_end, hipStream_t st) {
   const int g = a.nh / a.nkv, columns = a.nkv * ((g + 15) / 16);
