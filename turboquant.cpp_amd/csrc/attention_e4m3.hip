@@ -93,38 +93,63 @@ __device__ __forceinline__ void load_query(bf16x8 (&out)[PIECES], const act_t* r
 }
 __device__ __forceinline__ float group_max(float v) { return with_lane_xor<32>(with_lane_xor<16>(v, LanesMax()), LanesMax()); }
 __device__ __forceinline__ float group_sum(float v) { return with_lane_xor<32>(with_lane_xor<16>(v, LanesSum()), LanesSum()); }
-__device__ __forceinline__ float changed_score(float s, const ScoreMod& m, float r1, float r2, int dist) {
-#if defined(TQ_ACT_BF16)
-  return mod_score_fast(s, m.cap, m.r1 != nullptr, r1, r2, dist);
-#else
-  return mod_score(s, m.cap, m.r1 != nullptr, r1, r2, dist);
-#endif
+// Scores of a tile as the softmax takes them, and -inf where the column does not see the position, for one group of 16 columns.  MOD:
+// scaled, capped, biased, in units of log2; else (a positive scale alone) as the product left them, and the scale joins the exponent.
+// The cap in the bfloat16 library: cap tanh(x / cap) = cap - 2 cap / (e^(2 x / cap) + 1), which needs no bounds: e^.. may be 0 or infinite.
+struct Change {
+  float scale2, cap2, k2;      // scale, cap in units of log2; 2 log2(e) scale / cap
+};
+__device__ __forceinline__ Change change_of(const E4m3Attn& a) {
+  return Change{a.scale * LOG2E, a.mod.cap * LOG2E, a.mod.cap > 0.f ? 2.f * LOG2E * a.scale / a.mod.cap : 0.f};
 }
-
-// Scores of a tile to units of log2 and -inf where the column does not see the position, for one group of 16 columns.
 template <bool MOD>
-__device__ __forceinline__ void final_scores(f32x4 (&s)[4], const E4m3Attn& a, float r1, float r2, int pos0, int p, int lo, bool masked) {
+__device__ __forceinline__ void final_scores(f32x4 (&s)[4], const E4m3Attn& a, const Change& ch, float r1, float r2, int pos0, int p, int lo, bool masked) {
   const int c = (threadIdx.x % 64) / 16;
+  if constexpr (MOD) {
+#if defined(TQ_ACT_BF16)
+    if (a.mod.cap > 0.f) {
 #pragma unroll
-  for (int jt = 0; jt < 4; ++jt)
+      for (int jt = 0; jt < 4; ++jt)
 #pragma unroll
-    for (int v = 0; v < 4; ++v) {
-      const int key = pos0 + 16 * jt + 4 * c + v;
-      float x = s[jt][v] * (MOD ? a.scale : a.scale * LOG2E);
-      if constexpr (MOD) x = changed_score(x, a.mod, r1, r2, p - key) * LOG2E;
-      if (masked) x = key <= p && key >= lo ? x : -INFINITY;
-      s[jt][v] = x;
+        for (int v = 0; v < 4; ++v)
+          s[jt][v] = fmaf(-2.f * ch.cap2, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[jt][v] * ch.k2) + 1.f), ch.cap2);
+    } else {
+#pragma unroll
+      for (int jt = 0; jt < 4; ++jt) s[jt] *= ch.scale2;
     }
+    if (a.mod.r1)
+#pragma unroll
+      for (int jt = 0; jt < 4; ++jt)
+#pragma unroll
+        for (int v = 0; v < 4; ++v)
+          s[jt][v] -= r1 * __builtin_amdgcn_logf(fmaf(r2, (float)max(p - (pos0 + 16 * jt + 4 * c + v), 0), 1.f));
+#else
+#pragma unroll
+    for (int jt = 0; jt < 4; ++jt)
+#pragma unroll
+      for (int v = 0; v < 4; ++v)
+        s[jt][v] = mod_score(s[jt][v] * a.scale, a.mod.cap, a.mod.r1 != nullptr, r1, r2, p - (pos0 + 16 * jt + 4 * c + v)) * LOG2E;
+#endif
+  }
+  if (masked)
+#pragma unroll
+    for (int jt = 0; jt < 4; ++jt)
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        const int key = pos0 + 16 * jt + 4 * c + v;
+        s[jt][v] = key <= p && key >= lo ? s[jt][v] : -INFINITY;
+      }
 }
-// The part of a tile between its products for one group of 16 columns: scores in, probabilities as operands out.
+// The part of a tile between its products for one group of 16 columns: scores in, probabilities as operands out.  `scale2`: what is left
+// to multiply the scores by (final_scores), positive.
 template <int DT>
-__device__ __forceinline__ void softmax_tile(f32x4 (&s)[4], f32x4 (&o)[DT], float& m, float& l, bf16x8 (&pf)[2][PIECES]) {
+__device__ __forceinline__ void softmax_tile(f32x4 (&s)[4], f32x4 (&o)[DT], float& m, float& l, float scale2, bf16x8 (&pf)[2][PIECES]) {
   float top = -INFINITY;
 #pragma unroll
   for (int jt = 0; jt < 4; ++jt)
 #pragma unroll
     for (int v = 0; v < 4; ++v) top = fmaxf(top, s[jt][v]);
-  top = group_max(top);
+  top = group_max(top) * scale2;
   // (a column's own decision: whatever the wave's other columns hold, its sums are the same)
   const bool moves = top > m + 8.f || (m == -INFINITY && top > m);
   if (__any(moves)) {
@@ -142,7 +167,7 @@ __device__ __forceinline__ void softmax_tile(f32x4 (&s)[4], f32x4 (&o)[DT], floa
   for (int jt = 0; jt < 4; ++jt)
 #pragma unroll
     for (int v = 0; v < 4; ++v) {
-      s[jt][v] = __builtin_amdgcn_exp2f(s[jt][v] - use);
+      s[jt][v] = __builtin_amdgcn_exp2f(fmaf(s[jt][v], scale2, -use));
       sum += s[jt][v];
     }
   l += group_sum(sum);
@@ -186,6 +211,7 @@ struct DecodeWave {
   int kvh, p, lo, h, r, c;
   bool valid;
   float r1, r2;
+  Change ch;
   bf16x8 qf[2 * (DT / 4)][PIECES];
   u32x4 k[4][DT / 4], v[DT];
   f32x4 ks, vs;
@@ -203,6 +229,7 @@ struct DecodeWave {
     row = a.pages.table + (int64_t)a.slots[b] * a.pages.bt_stride;
     r1 = MOD && a.mod.r1 ? a.mod.r1[h] : 0.f;
     r2 = MOD && a.mod.r1 ? a.mod.r2[h] : 0.f;
+    ch = change_of(a);
     const act_t* qrow = a.q + ((int64_t)a.cu[b] * a.nh + h) * hd;
 #pragma unroll
     for (int s = 0; s < DT / 4; ++s)
@@ -262,14 +289,14 @@ struct DecodeWave {
         }
     }
     if (next >= 0) fetch_k(next);
-    final_scores<MOD>(s, a, r1, r2, pos0, p, lo, pos0 + E4M3_TILE - 1 > p || pos0 < lo);
+    final_scores<MOD>(s, a, ch, r1, r2, pos0, p, lo, pos0 + E4M3_TILE - 1 > p || pos0 < lo);
     if (a.scores && valid) {
       float* at = a.scores + ((int64_t)b * a.nh + h) * a.ld_scores + pos0 + 4 * c;
 #pragma unroll
-      for (int jt = 0; jt < 4; ++jt) *reinterpret_cast<f32x4*>(at + 16 * jt) = s[jt];
+      for (int jt = 0; jt < 4; ++jt) *reinterpret_cast<f32x4*>(at + 16 * jt) = MOD ? s[jt] : s[jt] * ch.scale2;
     }
     bf16x8 pf[2][PIECES];
-    softmax_tile<DT>(s, o, m, l, pf);
+    softmax_tile<DT>(s, o, m, l, MOD ? 1.f : ch.scale2, pf);
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
@@ -319,25 +346,25 @@ __device__ __forceinline__ void join_sums(const E4m3Attn& a, const float* part, 
 }
 // Joins the runs of one head and writes the output row; gives log2 of the row's sum.  Values are added in four strands by run, and the
 // strands at the end.  MINE: the wave shares the head with three others and takes strand `mine` (the strands meet in `strands`,
-// [4][256]); else it takes all four.
-template <bool MINE>
+// [4][256]); else it takes all four.  E: 64 dimensions that a head has at most.
+template <bool MINE, int E>
 __device__ __forceinline__ float join_runs(const E4m3Attn& a, const float* part, int stride, int beg, int end, int h, int64_t t, int mine, float* strands) {
   constexpr int NS = MINE ? 1 : 4, NJ = MINE ? 16 : 1;
   const int lane = threadIdx.x % 64, hd = a.pages.hd;
-  float v[NJ][4] = {};
+  float v[NJ][E] = {};
   // a strand's values of 64 runs are asked for before the factors are known
   auto ask = [&](int i0) {
 #pragma unroll
     for (int k = 0; k < NJ; ++k)
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
+      for (int e = 0; e < E; ++e)
         if (64 * e < hd && i0 + 4 * k + mine < end) v[k][e] = part[(int64_t)(i0 + 4 * k + mine) * stride + min(64 * e + lane, hd - 1)];
   };
   if constexpr (MINE) ask(beg);
   float m, l, w;
   join_sums(a, part, stride, beg, end, h, m, l, w);
   const float use = m == -INFINITY ? 0.f : m;
-  float acc[NS][4] = {};
+  float acc[NS][E] = {};
   for (int i0 = beg; i0 < end; i0 += 64) {
     if (i0 > beg) {
       w = i0 + lane < end ? __builtin_amdgcn_exp2f(part[(int64_t)(i0 + lane) * stride + hd] - use) : 0.f;
@@ -350,7 +377,7 @@ __device__ __forceinline__ float join_runs(const E4m3Attn& a, const float* part,
         if (4 * k + mine >= n) break;
         const float ws = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), 4 * k + mine));
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[0][e] = fmaf(ws, v[k][e], acc[0][e]);
+        for (int e = 0; e < E; ++e) acc[0][e] = fmaf(ws, v[k][e], acc[0][e]);
       }
     } else {
 #pragma unroll 2
@@ -360,7 +387,7 @@ __device__ __forceinline__ float join_runs(const E4m3Attn& a, const float* part,
           if (j + s >= n) break;
           const float ws = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), j + s));
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
+          for (int e = 0; e < E; ++e)
             if (64 * e < hd) acc[s][e] = fmaf(ws, part[(int64_t)(i0 + j + s) * stride + min(64 * e + lane, hd - 1)], acc[s][e]);
         }
       }
@@ -370,41 +397,46 @@ __device__ __forceinline__ float join_runs(const E4m3Attn& a, const float* part,
   act_t* out = a.out + (t * a.nh + h) * hd;
   if constexpr (MINE) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) strands[256 * mine + 64 * e + lane] = acc[0][e];
+    for (int e = 0; e < E; ++e) strands[256 * mine + 64 * e + lane] = acc[0][e];
     __syncthreads();
     const int d = threadIdx.x;
     if (d < hd) out[d] = from_f32<act_t>(((strands[d] + strands[256 + d]) + (strands[512 + d] + strands[768 + d])) * inv);
   } else {
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
+    for (int e = 0; e < E; ++e)
       if (64 * e + lane < hd) out[64 * e + lane] = from_f32<act_t>(((acc[0][e] + acc[1][e]) + (acc[2][e] + acc[3][e])) * inv);
   }
   return lse_of(m, l);
 }
-// A position's weight of one token: the sum over the g heads of a kv head, whose sums `lse` has.  `ask` first, for eight heads' scores.
+// The weights of one token that four neighbouring positions from j on (of one tile, a multiple of four) receive: sums over the g heads
+// of a kv head, whose sums `lse` has.  `ask` first, for eight heads' scores.
 struct WeightOf {
-  float s[8];
+  f32x4 s[8];
   __device__ __forceinline__ void ask(const E4m3Attn& a, int b, int kvh, int i0, int j) {
     const int g = a.nh / a.nkv;
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      if (i0 + i < g) s[i] = a.scores[((int64_t)b * a.nh + kvh * g + i0 + i) * a.ld_scores + j];
+      if (i0 + i < g) s[i] = *reinterpret_cast<const f32x4*>(a.scores + ((int64_t)b * a.nh + kvh * g + i0 + i) * a.ld_scores + j);
   }
-  __device__ __forceinline__ void add(const E4m3Attn& a, const int* row, int b, int kvh, int j, const float* lse) {
+  __device__ __forceinline__ void add(const E4m3Attn& a, const int* row, int b, int kvh, int j, int lo, int p, const float* lse) {
     const int g = a.nh / a.nkv;
     int in_page;
     const int64_t head = e4m3_head_of(a.pages, row, j / E4M3_TILE, kvh, in_page);
     if (head < 0) return;
-    float* to = a.pages.weight + head * a.pages.page_size + in_page * E4M3_TILE + j % E4M3_TILE;
-    const float was = *to;
-    float w = 0.f;
+    f32x4* to = reinterpret_cast<f32x4*>(a.pages.weight + head * a.pages.page_size + in_page * E4M3_TILE + j % E4M3_TILE);
+    const f32x4 was = *to;
+    f32x4 w = {0.f, 0.f, 0.f, 0.f};
     for (int i0 = 0; i0 < g; i0 += 8) {
       if (i0) ask(a, b, kvh, i0, j);
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        if (i0 + i < g) w += __builtin_amdgcn_exp2f(s[i] - lse[i0 + i]);
+        if (i0 + i < g)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) w[e] += __builtin_amdgcn_exp2f(s[i][e] - lse[i0 + i]);
     }
-    *to = was + w;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[e] = j + e >= lo && j + e <= p ? was[e] + w[e] : was[e];
+    *to = w;
   }
 };
 
@@ -427,8 +459,9 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(DT > 12 || D
   }
 }
 
-// Joins them: blocks 0 .. nh B - 1 a head each, four waves with a strand of its runs each; behind them, with weights, blocks of 256 positions of
-// one (sequence, kv head), which work the heads' sums out for themselves.
+// Joins them: blocks 0 .. nh B - 1 a head each, four waves with a strand of its runs each; behind them, with weights, blocks of 1,024 positions
+// of one (sequence, kv head), which work the heads' sums out for themselves.
+template <int E>
 __global__ __launch_bounds__(256) void e4m3_join_kernel(E4m3Attn a, int blocks_of_weights) {
   __shared__ float lds[4 * 256];
   const int stride = a.pages.hd + 2, g = a.nh / a.nkv, wave = threadIdx.x / 64, lane = threadIdx.x % 64;
@@ -439,13 +472,13 @@ __global__ __launch_bounds__(256) void e4m3_join_kernel(E4m3Attn a, int blocks_o
   const int beg = lo / E4M3_TILE / S, end = p / E4M3_TILE / S + 1;
   if (joins) {
     const int h = x % a.nh;
-    join_runs<true>(a, a.partial + ((int64_t)b * a.nh + h) * a.max_runs * stride, stride, beg, end, h, a.cu[b], wave, lds);
+    join_runs<true, E>(a, a.partial + ((int64_t)b * a.nh + h) * a.max_runs * stride, stride, beg, end, h, a.cu[b], wave, lds);
     return;
   }
-  const int kvh = x / blocks_of_weights % a.nkv, j = x % blocks_of_weights * 256 + (int)threadIdx.x;
-  if (j - (int)threadIdx.x > p || j - (int)threadIdx.x + 255 < lo) return;
+  const int kvh = x / blocks_of_weights % a.nkv, j0 = x % blocks_of_weights * 1024, j = j0 + 4 * (int)threadIdx.x;
+  if (j0 > p || j0 + 1023 < lo) return;
   const int* row = a.pages.table + (int64_t)a.slots[b] * a.pages.bt_stride;
-  const bool has = j >= lo && j <= p;
+  const bool has = j + 3 >= lo && j <= p;
   WeightOf of;
   if (has) of.ask(a, b, kvh, 0, j);
 #pragma unroll 2
@@ -456,7 +489,7 @@ __global__ __launch_bounds__(256) void e4m3_join_kernel(E4m3Attn a, int blocks_o
     if (lane == 0) lds[i] = lse_of(m, l);
   }
   __syncthreads();
-  if (has) of.add(a, row, b, kvh, j, lds);
+  if (has) of.add(a, row, b, kvh, j, lo, p, lds);
 }
 
 // A step whose sequences all hold at most SHORT_END positions: grid (nkv * ceil(g / 16), B), one launch.
@@ -478,16 +511,16 @@ __global__ __launch_bounds__(64 * SHORT_WAVES) __attribute__((amdgpu_waves_per_e
   }
   __syncthreads();
   for (int i = wave; i < heads; i += SHORT_WAVES) {
-    const float x = join_runs<false>(a, sums + i * stride, heads * stride, 0, end - beg, kvh * g + 16 * cg + i, a.cu[b], -1, nullptr);
+    const float x = join_runs<false, DT <= 8 ? 2 : 4>(a, sums + i * stride, heads * stride, 0, end - beg, kvh * g + 16 * cg + i, a.cu[b], -1, nullptr);
     if (lane == 0) lse[i] = x;
   }
   if (!a.scores) return;
   __threadfence_block();      // (the scores that the workgroup's waves have written)
   __syncthreads();
-  for (int j = max(w.lo, beg * E4M3_TILE) + (int)threadIdx.x; j <= w.p; j += 64 * SHORT_WAVES) {
+  for (int j = w.lo / 4 * 4 + 4 * (int)threadIdx.x; j <= w.p; j += 256 * SHORT_WAVES) {
     WeightOf of;
     of.ask(a, b, kvh, 0, j);
-    of.add(a, w.row, b, kvh, j, lse);
+    of.add(a, w.row, b, kvh, j, w.lo, w.p, lse);
   }
 }
 
@@ -504,6 +537,7 @@ template <int DT, int QG, bool MOD>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DT > 8 ? 1 : 2))) void e4m3_prompt_kernel(E4m3Attn a, int n_blocks) {
   extern __shared__ __attribute__((aligned(16))) __bf16 tiles[];
   constexpr int KS = DT / 2, CH = (E4M3_TILE * DT + 255) / 256, BUF = 2 * E4M3_TILE * 16 * DT;
+  constexpr bool AHEAD = DT <= 8 && PIECES == 1;
   const int per_block = a.nh * a.B, hd = a.pages.hd;
   const int blk = n_blocks - 1 - (int)blockIdx.x / per_block, h = (int)blockIdx.x % per_block % a.nh, b = (int)blockIdx.x % per_block / a.nh;
   const int tid = threadIdx.x, lane = tid % 64, r = lane % 16, c = lane / 16, wave = __builtin_amdgcn_readfirstlane(tid / 64);
@@ -512,6 +546,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DT > 8 ? 1 
   const int start = a.start[b], kvh = h / (a.nh / a.nkv);
   const int* row = a.pages.table + (int64_t)a.slots[b] * a.pages.bt_stride;
   const float r1 = MOD && a.mod.r1 ? a.mod.r1[h] : 0.f, r2 = MOD && a.mod.r1 ? a.mod.r2[h] : 0.f;
+  const Change ch = change_of(a);
   bf16x8 qf[QG][KS][PIECES];
   f32x4 o[QG][DT];
   float m[QG], l[QG];
@@ -590,36 +625,56 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DT > 8 ? 1 
       const __bf16 *Ks = tiles + cur, *Vs = Ks + E4M3_TILE * 16 * DT;
       const int pos0 = tile * E4M3_TILE;
       const bool masked = pos0 + E4M3_TILE - 1 > first || pos0 < lo_last;
+      // Operands are asked for ahead of their products, as many as there are registers for: half of the keys before the first product, the
+      // other half during it, the first values before the softmax.
+      bf16x8 kf[4][KS], vf[2][DT];
       f32x4 s[QG][4];
+      auto ask_k = [&](int jt) {
 #pragma unroll
-      for (int jt = 0; jt < 4; ++jt) {
+        for (int ks = 0; ks < KS; ++ks) kf[jt][ks] = *reinterpret_cast<const bf16x8*>(Ks + k_at<DT>(16 * jt + r, 4 * ks + c));
+      };
+      auto scores = [&](int jt) {
 #pragma unroll
         for (int g = 0; g < QG; ++g) s[g][jt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-          const bf16x8 kf = *reinterpret_cast<const bf16x8*>(Ks + k_at<DT>(16 * jt + r, 4 * ks + c));
+        for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
           for (int g = 0; g < QG; ++g)
 #pragma unroll
-            for (int pc = PIECES - 1; pc >= 0; --pc) s[g][jt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[g][ks][pc], s[g][jt], 0, 0, 0);
-        }
-      }
+            for (int pc = PIECES - 1; pc >= 0; --pc) s[g][jt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[jt][ks], qf[g][ks][pc], s[g][jt], 0, 0, 0);
+      };
+      auto ask_v = [&](int pr) {
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) vf[pr][dt] = *reinterpret_cast<const bf16x8*>(Vs + v_at(16 * dt + r, 2 * c + pr));
+      };
+      ask_k(0);
+      ask_k(1);
+      if constexpr (AHEAD) __builtin_amdgcn_sched_barrier(0);
+      ask_k(2);
+      scores(0);
+      ask_k(3);
+      scores(1);
+      if constexpr (AHEAD) __builtin_amdgcn_sched_barrier(0);
+      scores(2);
+      scores(3);
+      ask_v(0);
+      if constexpr (AHEAD) __builtin_amdgcn_sched_barrier(0);
       bf16x8 pf[QG][2][PIECES];
 #pragma unroll
       for (int g = 0; g < QG; ++g) {
-        final_scores<MOD>(s[g], a, r1, r2, pos0, p[g], lo[g], masked);
-        softmax_tile<DT>(s[g], o[g], m[g], l[g], pf[g]);
+        final_scores<MOD>(s[g], a, ch, r1, r2, pos0, p[g], lo[g], masked);
+        softmax_tile<DT>(s[g], o[g], m[g], l[g], MOD ? 1.f : ch.scale2, pf[g]);
       }
+      ask_v(1);
+      if constexpr (AHEAD) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
+      for (int pr = 0; pr < 2; ++pr)
 #pragma unroll
-        for (int pr = 0; pr < 2; ++pr) {
-          const bf16x8 vf = *reinterpret_cast<const bf16x8*>(Vs + v_at(16 * dt + r, 2 * c + pr));
+        for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
           for (int g = 0; g < QG; ++g)
 #pragma unroll
-            for (int pc = PIECES - 1; pc >= 0; --pc) o[g][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[g][pr][pc], o[g][dt], 0, 0, 0);
-        }
+            for (int pc = PIECES - 1; pc >= 0; --pc) o[g][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[pr][dt], pf[g][pr][pc], o[g][dt], 0, 0, 0);
     }
     __syncthreads();
   }
@@ -643,40 +698,36 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DT > 8 ? 1 
   }
 }
 
-template <int DT>
-struct TileKeys {
-  u32x4 k[4][DT / 4];
-  f32x4 ks;
-};
-template <int DT>
-__device__ __forceinline__ void fetch_keys(TileKeys<DT>& t, const E4m3Pages& p, const int* row, int tile, int kvh) {
-  const int lane = threadIdx.x % 64, r = lane % 16, c = lane / 16;
-  int in_page;
-  int64_t head = e4m3_head_of(p, row, tile, kvh, in_page);
-  if (head < 0) head = 0;
-  const uint8_t* at = p.k + e4m3_tile_at(p, head, in_page);
-  t.ks = *reinterpret_cast<const f32x4*>(p.k_scale + e4m3_scale_at(p, head, in_page));
-#pragma unroll
-  for (int ks = 0; ks < DT / 4; ++ks) {
-    const int ch = min(4 * ks + c, p.hd / 16 - 1);
-#pragma unroll
-    for (int jt = 0; jt < 4; ++jt) t.k[jt][ks] = *reinterpret_cast<const u32x4*>(at + ch * 1024 + (16 * jt + r) * 16);
-  }
-}
 // The weights that a prompt gives its positions, from the scores once more and the rows' sums: grid (tiles, nkv, B), block 256.  A
 // workgroup keeps a tile's keys in registers and goes through the tokens that may see it and the heads of its kv head, 16 tokens of one
 // head to a wave at a time; one sum over lanes and waves at the end, in a fixed order.
 template <int DT, bool MOD>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DT > 8 ? 1 : 2))) void e4m3_prompt_weights_kernel(E4m3Attn a) {
+  constexpr int KS = 2 * (DT / 4);
   __shared__ float sums[4][E4M3_TILE];
   const int kvh = blockIdx.y, b = blockIdx.z, g = a.nh / a.nkv, hd = a.pages.hd;
   const int tid = threadIdx.x, lane = tid % 64, r = lane % 16, c = lane / 16, wave = __builtin_amdgcn_readfirstlane(tid / 64);
   const int t0 = a.cu[b], n = a.cu[b + 1] - t0, start = a.start[b];
   const int tile = reach_lo(start, a.window, a.mod.chunk) / E4M3_TILE + (int)blockIdx.x, pos0 = tile * E4M3_TILE;
   if (n <= 0 || pos0 >= start + n) return;
-  TileKeys<DT> t;
   const int* row = a.pages.table + (int64_t)a.slots[b] * a.pages.bt_stride;
-  fetch_keys<DT>(t, a.pages, row, tile, kvh);
+  const Change ch = change_of(a);
+  int in_page;
+  int64_t head = e4m3_head_of(a.pages, row, tile, kvh, in_page);
+  if (head < 0) return;
+  bf16x8 kf[4][KS];
+  {
+    const uint8_t* at = a.pages.k + e4m3_tile_at(a.pages, head, in_page);
+    const f32x4 scale = *reinterpret_cast<const f32x4*>(a.pages.k_scale + e4m3_scale_at(a.pages, head, in_page));
+#pragma unroll
+    for (int i = 0; i < KS / 2; ++i)
+#pragma unroll
+      for (int jt = 0; jt < 4; ++jt) {
+        const u32x4 w = *reinterpret_cast<const u32x4*>(at + min(4 * i + c, hd / 16 - 1) * 1024 + (16 * jt + r) * 16);
+        kf[jt][2 * i] = numbers(w[0], w[1], scale[jt]);
+        kf[jt][2 * i + 1] = numbers(w[2], w[3], scale[jt]);
+      }
+  }
   // the tokens that may see a position of the tile: from the tile's first to the last whose reach has its last
   const int from = max(pos0 - start, 0) / 16;
   int to = n;
@@ -686,34 +737,38 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DT > 8 ? 1 
   f32x4 acc[4];
 #pragma unroll
   for (int jt = 0; jt < 4; ++jt) acc[jt] = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int i = wave; i < items; i += 4) {
+  bf16x8 qf[KS][PIECES];
+  float lse;
+  auto ask = [&](int i) {
     const int h = kvh * g + i % g, qi = (from + i / g) * 16 + r;
-    const bool valid = qi < n;
-    const int p = valid ? start + qi : -1, lo = reach_lo(p, a.window, a.mod.chunk);
-    const int64_t at = (int64_t)(t0 + (valid ? qi : 0)) * a.nh + h;
-    const float lse = a.lse[at];
+    const int64_t at = (int64_t)(t0 + min(qi, n - 1)) * a.nh + h;
+    lse = a.lse[at];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) load_query(qf[ks], a.q + at * hd, 64 * (ks / 2) + 16 * c + 8 * (ks % 2), hd, true);
+  };
+  if (wave < items) ask(wave);
+  for (int i = wave; i < items; i += 4) {
+    const int h = kvh * g + i % g, q0 = (from + i / g) * 16, qi = q0 + r;
+    const int p = qi < n ? start + qi : -1, lo = reach_lo(p, a.window, a.mod.chunk);
     const float r1 = MOD && a.mod.r1 ? a.mod.r1[h] : 0.f, r2 = MOD && a.mod.r1 ? a.mod.r2[h] : 0.f;
     f32x4 s[4];
 #pragma unroll
     for (int jt = 0; jt < 4; ++jt) s[jt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int ks = 0; ks < DT / 4; ++ks)
+    for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        bf16x8 qf[PIECES];
-        load_query(qf, a.q + at * hd, 64 * ks + 16 * c + 8 * half, hd, valid);
+      for (int jt = 0; jt < 4; ++jt)
 #pragma unroll
-        for (int jt = 0; jt < 4; ++jt) {
-          const bf16x8 kf = numbers(t.k[jt][ks][2 * half], t.k[jt][ks][2 * half + 1], t.ks[jt]);
-#pragma unroll
-          for (int pc = PIECES - 1; pc >= 0; --pc) s[jt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[pc], s[jt], 0, 0, 0);
-        }
-      }
-    final_scores<MOD>(s, a, r1, r2, pos0, p, lo, true);
+        for (int pc = PIECES - 1; pc >= 0; --pc) s[jt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[jt][ks], qf[ks][pc], s[jt], 0, 0, 0);
+    const float sum = lse;
+    if (i + 4 < items) ask(i + 4);      // (the next queries travel during the powers)
+    // every token of the 16 sees the whole tile: nothing to compare
+    const bool masked = q0 + 15 >= n || start + q0 < pos0 + E4M3_TILE - 1 || reach_lo(start + q0 + 15, a.window, a.mod.chunk) > pos0;
+    final_scores<MOD>(s, a, ch, r1, r2, pos0, p, lo, masked);
 #pragma unroll
     for (int jt = 0; jt < 4; ++jt)
 #pragma unroll
-      for (int v = 0; v < 4; ++v) acc[jt][v] += __builtin_amdgcn_exp2f(s[jt][v] - lse);
+      for (int v = 0; v < 4; ++v) acc[jt][v] += __builtin_amdgcn_exp2f(fmaf(s[jt][v], MOD ? 1.f : ch.scale2, -sum));
   }
 #pragma unroll
   for (int jt = 0; jt < 4; ++jt)
@@ -724,10 +779,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DT > 8 ? 1 
     }
   __syncthreads();
   if (tid < E4M3_TILE && pos0 + tid < start + n) {
-    int in_page;
-    const int64_t head = e4m3_head_of(a.pages, row, tile, kvh, in_page);
-    if (head >= 0)
-      a.pages.weight[head * a.pages.page_size + in_page * E4M3_TILE + tid] += (sums[0][tid] + sums[1][tid]) + (sums[2][tid] + sums[3][tid]);
+    a.pages.weight[head * a.pages.page_size + in_page * E4M3_TILE + tid] += (sums[0][tid] + sums[1][tid]) + (sums[2][tid] + sums[3][tid]);
   }
 }
 
@@ -747,9 +799,9 @@ static int launch_decode(const E4m3Attn& a, int max_end, hipStream_t st) {
   }
   const int waves = min(a.max_runs, max(1, DECODE_WAVES / (columns * a.B)));
   hipLaunchKernelGGL((e4m3_decode_kernel<DT, MOD>), dim3(waves, columns, a.B), dim3(64), 0, st, a);
-  const int blocks = a.scores ? (max_end + 255) / 256 : 0;
+  const int blocks = a.scores ? (max_end + 1023) / 1024 : 0;
   if ((int64_t)a.nh * a.B + (int64_t)blocks * a.nkv * a.B > 0xFFFFFF) return TQ_ERR_UNSUPPORTED;
-  hipLaunchKernelGGL(e4m3_join_kernel, dim3(a.nh * a.B + blocks * a.nkv * a.B), dim3(256), 0, st, a, blocks);
+  hipLaunchKernelGGL(e4m3_join_kernel<DT <= 8 ? 2 : 4>, dim3(a.nh * a.B + blocks * a.nkv * a.B), dim3(256), 0, st, a, blocks);
   return 0;
 }
 template <int DT, int QG, bool MOD>
@@ -775,7 +827,7 @@ static int launch_as(const E4m3Attn& a, int decode, int max_new, int max_end, hi
 }
 template <int DT>
 static int launch(const E4m3Attn& a, int decode, int max_new, int max_end, hipStream_t st) {
-  return a.mod.cap > 0.f || a.mod.r1 ? launch_as<DT, true>(a, decode, max_new, max_end, st) : launch_as<DT, false>(a, decode, max_new, max_end, st);
+  return a.mod.cap > 0.f || a.mod.r1 || !(a.scale > 0.f) ? launch_as<DT, true>(a, decode, max_new, max_end, st) : launch_as<DT, false>(a, decode, max_new, max_end, st);
 }
 
 // Floats of scratch: for decoding the runs' sums, with weights the scores too; for prompts with weights the rows' sums.
