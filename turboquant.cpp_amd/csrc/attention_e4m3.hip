@@ -16,6 +16,7 @@
 // at every tile; probabilities are then at most 256, which neither type minds.
 #include "cache_e4m3.h"
 #include "score_mod.h"
+#include <stdlib.h>
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
@@ -131,7 +132,8 @@ __device__ __forceinline__ void final_scores(f32x4 (&s)[4], const E4m3Attn& a, c
         s[jt][v] = mod_score(s[jt][v] * a.scale, a.mod.cap, a.mod.r1 != nullptr, r1, r2, p - (pos0 + 16 * jt + 4 * c + v)) * LOG2E;
 #endif
   }
-  if (masked)
+  if (masked) {
+    asm volatile("");      // (a branch: as conditions the comparisons would be a third of the instructions of tiles that need none)
 #pragma unroll
     for (int jt = 0; jt < 4; ++jt)
 #pragma unroll
@@ -139,9 +141,10 @@ __device__ __forceinline__ void final_scores(f32x4 (&s)[4], const E4m3Attn& a, c
         const int key = pos0 + 16 * jt + 4 * c + v;
         s[jt][v] = key <= p && key >= lo ? s[jt][v] : -INFINITY;
       }
+  }
 }
 // The part of a tile between its products for one group of 16 columns: scores in, probabilities as operands out.  `scale2`: what is left
-// to multiply the scores by (final_scores), positive.
+// to multiply the scores by (final_scores), positive.  l is the lane's share of a column's sum: the four lanes' shares are added at the end.
 template <int DT>
 __device__ __forceinline__ void softmax_tile(f32x4 (&s)[4], f32x4 (&o)[DT], float& m, float& l, float scale2, bf16x8 (&pf)[2][PIECES]) {
   float top = -INFINITY;
@@ -170,7 +173,7 @@ __device__ __forceinline__ void softmax_tile(f32x4 (&s)[4], f32x4 (&o)[DT], floa
       s[jt][v] = __builtin_amdgcn_exp2f(fmaf(s[jt][v], scale2, -use));
       sum += s[jt][v];
     }
-  l += group_sum(sum);
+  l += sum;
 #pragma unroll
   for (int pr = 0; pr < 2; ++pr) {
     const float x[8] = {s[2 * pr][0], s[2 * pr][1], s[2 * pr][2], s[2 * pr][3], s[2 * pr + 1][0], s[2 * pr + 1][1], s[2 * pr + 1][2], s[2 * pr + 1][3]};
@@ -310,6 +313,7 @@ struct DecodeWave {
   }
   // A run's sums to its place, and a new run.
   __device__ __forceinline__ void leave(float* out) {
+    l = group_sum(l);
     if (valid) {
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt)
@@ -533,14 +537,17 @@ template <int DT>
 __device__ __forceinline__ int k_at(int row, int ch) { return row * (16 * DT) + ((ch ^ (row & (DT % 8 == 0 ? 15 : 7))) << 3); }
 __device__ __forceinline__ int v_at(int d, int ch) { return d * E4M3_TILE + ((ch ^ (d & 7)) << 3); }
 
-template <int DT, int QG, bool MOD>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DT > 8 ? 1 : 2))) void e4m3_prompt_kernel(E4m3Attn a, int n_blocks) {
+// HALVES 2: twice the waves, and tiles by turns: four waves take the first, third, .. tile, the other four the others, for the same tokens;
+// their sums meet in LDS at the end.  For prompts with few workgroups, whose last blocks' tiles would else follow one another on a chip that is mostly idle.
+template <int DT, int QG, bool MOD, int HALVES>
+__global__ __launch_bounds__(256 * HALVES) __attribute__((amdgpu_waves_per_eu(DT > 8 ? 1 : 2))) void e4m3_prompt_kernel(E4m3Attn a, int n_blocks) {
   extern __shared__ __attribute__((aligned(16))) __bf16 tiles[];
   constexpr int KS = DT / 2, CH = (E4M3_TILE * DT + 255) / 256, BUF = 2 * E4M3_TILE * 16 * DT;
   constexpr bool AHEAD = DT <= 8 && PIECES == 1;
   const int per_block = a.nh * a.B, hd = a.pages.hd;
   const int blk = n_blocks - 1 - (int)blockIdx.x / per_block, h = (int)blockIdx.x % per_block % a.nh, b = (int)blockIdx.x % per_block / a.nh;
-  const int tid = threadIdx.x, lane = tid % 64, r = lane % 16, c = lane / 16, wave = __builtin_amdgcn_readfirstlane(tid / 64);
+  const int half = HALVES == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / 256);
+  const int tid = threadIdx.x % 256, lane = tid % 64, r = lane % 16, c = lane / 16, wave = __builtin_amdgcn_readfirstlane(tid / 64);
   const int t0 = a.cu[b], n = a.cu[b + 1] - t0, qb = blk * 64 * QG;
   if (qb >= n) return;
   const int start = a.start[b], kvh = h / (a.nh / a.nkv);
@@ -562,8 +569,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DT > 8 ? 1 
     for (int ks = 0; ks < KS; ++ks) load_query(qf[g][ks], qrow, 32 * ks + 8 * c, hd, valid);
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) o[g][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
-    m[g] = a.mod.sink ? a.mod.sink[h] * LOG2E : -INFINITY;
-    l[g] = a.mod.sink && m[g] != -INFINITY ? 1.f : 0.f;
+    m[g] = a.mod.sink && half == 0 ? a.mod.sink[h] * LOG2E : -INFINITY;
+    l[g] = m[g] != -INFINITY && c == 0 ? 1.f : 0.f;      // (the sink counts once)
   }
   const int wg_last = start + min(qb + 64 * QG, n) - 1;
   const int tile_beg = reach_lo(start + qb, a.window, a.mod.chunk) / E4M3_TILE, tile_end = wg_last / E4M3_TILE + 1;
@@ -606,23 +613,28 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DT > 8 ? 1 
       }
     }
   };
+  __bf16* mine = tiles + half * 2 * BUF;
   // what lies behind a head's end in LDS is read against zeros of the queries (keys) or not stored (values): it has to be finite
   if (hd < 16 * DT) {
-    for (int i = tid; i < 2 * BUF / 8; i += 256) *reinterpret_cast<bf16x8*>(tiles + 8 * i) = nothing();
+    for (int i = tid; i < 2 * BUF / 8; i += 256) *reinterpret_cast<bf16x8*>(mine + 8 * i) = nothing();
     __syncthreads();
   }
-  fetch_tile(tile_beg);
-  stage(tiles);
-  if (tile_beg + 1 < tile_end) fetch_tile(tile_beg + 1);
+  const int tile0 = tile_beg + half;
+  if (tile0 < tile_end) {
+    fetch_tile(tile0);
+    stage(mine);
+    if (tile0 + HALVES < tile_end) fetch_tile(tile0 + HALVES);
+  }
   __syncthreads();
   int cur = 0;
-  for (int tile = tile_beg; tile < tile_end; ++tile, cur ^= BUF) {
-    if (tile + 1 < tile_end) {
-      stage(tiles + (cur ^ BUF));
-      if (tile + 2 < tile_end) fetch_tile(tile + 2);
+  for (int at = tile_beg; at < tile_end; at += HALVES, cur ^= BUF) {      // (as often for either half)
+    const int tile = at + half;
+    if (tile + HALVES < tile_end) {
+      stage(mine + (cur ^ BUF));
+      if (tile + 2 * HALVES < tile_end) fetch_tile(tile + 2 * HALVES);
     }
     if (tile >= wave_beg && tile < wave_end) {
-      const __bf16 *Ks = tiles + cur, *Vs = Ks + E4M3_TILE * 16 * DT;
+      const __bf16 *Ks = mine + cur, *Vs = Ks + E4M3_TILE * 16 * DT;
       const int pos0 = tile * E4M3_TILE;
       const bool masked = pos0 + E4M3_TILE - 1 > first || pos0 < lo_last;
       // Operands are asked for ahead of their products, as many as there are registers for: half of the keys before the first product, the
@@ -677,6 +689,37 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DT > 8 ? 1 
             for (int pc = PIECES - 1; pc >= 0; --pc) o[g][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[pr][dt], pf[g][pr][pc], o[g][dt], 0, 0, 0);
     }
     __syncthreads();
+  }
+#pragma unroll
+  for (int g = 0; g < QG; ++g) l[g] = group_sum(l[g]);
+  if constexpr (HALVES == 2) {
+    static_assert(QG * DT * 4 * 64 * 16 + QG * 4 * 64 * 8 <= 2 * HALVES * BUF * 2, "the second half's sums fit into the tiles' place");
+    f32x4* sums = reinterpret_cast<f32x4*>(tiles);
+    float2* ml = reinterpret_cast<float2*>(sums + 4 * QG * DT * 64);
+    if (half == 1) {
+#pragma unroll
+      for (int g = 0; g < QG; ++g) {
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) sums[((wave * QG + g) * DT + dt) * 64 + lane] = o[g][dt];
+        ml[(wave * QG + g) * 64 + lane] = make_float2(m[g], l[g]);
+      }
+    }
+    __syncthreads();
+    if (half == 1) return;
+#pragma unroll
+    for (int g = 0; g < QG; ++g) {
+      const float2 other = ml[(wave * QG + g) * 64 + lane];
+      const float to = fmaxf(m[g], other.x), use = to == -INFINITY ? 0.f : to;
+      const float mine_by = __builtin_amdgcn_exp2f(m[g] - use), other_by = __builtin_amdgcn_exp2f(other.x - use);
+      l[g] = fmaf(other.y, other_by, l[g] * mine_by);
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) {
+        const f32x4 x = sums[((wave * QG + g) * DT + dt) * 64 + lane];
+#pragma unroll
+        for (int v = 0; v < 4; ++v) o[g][dt][v] = fmaf(x[v], other_by, o[g][dt][v] * mine_by);
+      }
+      m[g] = to;
+    }
   }
 #pragma unroll
   for (int g = 0; g < QG; ++g) {
@@ -804,22 +847,29 @@ static int launch_decode(const E4m3Attn& a, int max_end, hipStream_t st) {
   hipLaunchKernelGGL(e4m3_join_kernel<DT <= 8 ? 2 : 4>, dim3(a.nh * a.B + blocks * a.nkv * a.B), dim3(256), 0, st, a, blocks);
   return 0;
 }
-template <int DT, int QG, bool MOD>
+template <int DT, int QG, bool MOD, int HALVES>
 static int launch_prompt(const E4m3Attn& a, int max_new, hipStream_t st) {
-  const size_t shmem = 2 * (size_t)2 * E4M3_TILE * 16 * DT * sizeof(__bf16);
-  const hipError_t e = hipFuncSetAttribute((const void*)e4m3_prompt_kernel<DT, QG, MOD>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)shmem);
-  if (e != hipSuccess) return (int)e;
+  const size_t shmem = HALVES * 2 * (size_t)2 * E4M3_TILE * 16 * DT * sizeof(__bf16);
+  if (shmem > 64 * 1024) {
+    const hipError_t e = hipFuncSetAttribute((const void*)e4m3_prompt_kernel<DT, QG, MOD, HALVES>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)shmem);
+    if (e != hipSuccess) return (int)e;
+  }
   const int n_blocks = (max_new + 64 * QG - 1) / (64 * QG);
-  if ((int64_t)n_blocks * a.nh * a.B > 0xFFFFFF) return TQ_ERR_UNSUPPORTED;      // (a launch's threads are counted in 32 bits)
-  hipLaunchKernelGGL((e4m3_prompt_kernel<DT, QG, MOD>), dim3(n_blocks * a.nh * a.B), dim3(256), shmem, st, a, n_blocks);
+  if ((int64_t)n_blocks * a.nh * a.B > 0x7FFFFF) return TQ_ERR_UNSUPPORTED;      // (a launch's threads are counted in 32 bits)
+  hipLaunchKernelGGL((e4m3_prompt_kernel<DT, QG, MOD, HALVES>), dim3(n_blocks * a.nh * a.B), dim3(256 * HALVES), shmem, st, a, n_blocks);
   return 0;
 }
 template <int DT, bool MOD>
 static int launch_as(const E4m3Attn& a, int decode, int max_new, int max_end, hipStream_t st) {
   if (decode) return launch_decode<DT, MOD>(a, max_end, st);
-  // two groups of 16 tokens to a wave halve the reads from LDS, where that leaves the chip two workgroups to a compute unit
-  const bool two = PIECES == 1 && DT <= 8 && (int64_t)((max_new + 127) / 128) * a.nh * a.B >= 512;
-  const int rc = two ? launch_prompt<DT, (PIECES == 1 && DT <= 8) ? 2 : 1, MOD>(a, max_new, st) : launch_prompt<DT, 1, MOD>(a, max_new, st);
+  // two groups of 16 tokens to a wave halve the reads from LDS, where that leaves the chip a workgroup to a compute unit
+  constexpr int TWO = PIECES == 1 && DT <= 8 ? 2 : 1, HALVES = DT <= 8 ? 2 : 1;
+  const char* e1 = getenv("TQ_T1"); const char* e2 = getenv("TQ_T2");
+  const int64_t of_two = (int64_t)((max_new + 127) / 128) * a.nh * a.B;
+  int rc;
+  const bool two = TWO == 2 && of_two >= (e1 ? atoi(e1) : 192), halves = (TWO == 2 && two ? of_two : (int64_t)((max_new + 63) / 64) * a.nh * a.B) <= (e2 ? atoi(e2) : 512);
+  if (two) rc = halves ? launch_prompt<DT, TWO, MOD, HALVES>(a, max_new, st) : launch_prompt<DT, TWO, MOD, 1>(a, max_new, st);
+  else rc = halves ? launch_prompt<DT, 1, MOD, HALVES>(a, max_new, st) : launch_prompt<DT, 1, MOD, 1>(a, max_new, st);
   if (rc) return rc;
   if (a.lse)
     hipLaunchKernelGGL((e4m3_prompt_weights_kernel<DT, MOD>), dim3((max_end + E4M3_TILE - 1) / E4M3_TILE, a.nkv, a.B), dim3(256), 0, st, a);
