@@ -16,7 +16,6 @@
 // at every tile; probabilities are then at most 256, which neither type minds.
 #include "cache_e4m3.h"
 #include "score_mod.h"
-#include <stdlib.h>
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
@@ -41,7 +40,8 @@ struct E4m3Attn {
   ScoreMod mod;
   float* partial;               // decoding: [B][nh][max_runs][hd + 2]
   int max_runs;
-  float* scores;                // decoding with weights: [B][nh][ld_scores], a column's scores in units of log2
+  float* scores;                // with weights: decoding [B][nh][ld_scores], a column's scores in units of log2; prompts [B][cuts][nh][ld_scores], a
+                                // cut's sums of probabilities
   int64_t ld_scores;
   float* lse;                   // prompts with weights: [T][nh] log2 of a row's sum of 2^score, the sink's included
   E4m3Pages pages;
@@ -741,25 +741,34 @@ __global__ __launch_bounds__(256 * HALVES) __attribute__((amdgpu_waves_per_eu(DT
   }
 }
 
-// The weights that a prompt gives its positions, from the scores once more and the rows' sums: grid (tiles, nkv, B), block 256.  A
-// workgroup keeps a tile's keys in registers and goes through the tokens that may see it and the heads of its kv head, 16 tokens of one
-// head to a wave at a time; one sum over lanes and waves at the end, in a fixed order.
+// The weights that a prompt gives its positions, from the scores once more and the rows' sums: grid (tiles / 4, nh, B * cuts), block 256.  A
+// wave keeps a tile's keys in registers, as numbers; the workgroup goes through the tokens of its cut that may see one of its four
+// tiles, 32 at a time, which come through LDS once for the four waves (each wave for itself asked the caches for 4 KiB of queries
+// for every 16 products, and waited: 166 us for 4,096 tokens of 28 heads).  A wave sums its own columns, in order, and at the end
+// over lanes; a second kernel adds the columns' sums over cuts and a kv head's heads.
+#define WEIGHT_TOKENS 32
 template <int DT, bool MOD>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DT > 8 ? 1 : 2))) void e4m3_prompt_weights_kernel(E4m3Attn a) {
-  constexpr int KS = 2 * (DT / 4);
-  __shared__ float sums[4][E4M3_TILE];
-  const int kvh = blockIdx.y, b = blockIdx.z, g = a.nh / a.nkv, hd = a.pages.hd;
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DT * PIECES > 8 ? (DT * PIECES > 16 ? 1 : 2) : 3))) void e4m3_prompt_weights_kernel(E4m3Attn a, int cuts, int cut) {
+  constexpr int KS = 2 * (DT / 4), PITCH = 16 * DT + 16 / (int)sizeof(act_t), PER = 16 / (int)sizeof(act_t);      // (numbers to 16 bytes)
+  constexpr int CH = (WEIGHT_TOKENS * 16 * DT / PER + 255) / 256;
+  extern __shared__ __attribute__((aligned(16))) act_t qs[];      // [2][32][PITCH]
+  __shared__ float lses[2][WEIGHT_TOKENS];
+  const int h = blockIdx.y, kvh = h / (a.nh / a.nkv), b = blockIdx.z / cuts, hd = a.pages.hd;
   const int tid = threadIdx.x, lane = tid % 64, r = lane % 16, c = lane / 16, wave = __builtin_amdgcn_readfirstlane(tid / 64);
   const int t0 = a.cu[b], n = a.cu[b + 1] - t0, start = a.start[b];
-  const int tile = reach_lo(start, a.window, a.mod.chunk) / E4M3_TILE + (int)blockIdx.x, pos0 = tile * E4M3_TILE;
-  if (n <= 0 || pos0 >= start + n) return;
+  const int q_beg = (int)(blockIdx.z % cuts) * cut, q_end = min(q_beg + cut, n);      // (cut: a multiple of 32)
+  const int tile0 = reach_lo(start, a.window, a.mod.chunk) / E4M3_TILE + 4 * (int)blockIdx.x, tile = tile0 + wave;
+  if (n <= 0 || tile0 * E4M3_TILE >= start + n) return;
+  const int pos0 = tile * E4M3_TILE;
+  const bool has = pos0 < start + n;
   const int* row = a.pages.table + (int64_t)a.slots[b] * a.pages.bt_stride;
   const Change ch = change_of(a);
-  int in_page;
-  int64_t head = e4m3_head_of(a.pages, row, tile, kvh, in_page);
-  if (head < 0) return;
+  const float r1 = MOD && a.mod.r1 ? a.mod.r1[h] : 0.f, r2 = MOD && a.mod.r1 ? a.mod.r2[h] : 0.f;
   bf16x8 kf[4][KS];
   {
+    int in_page;
+    int64_t head = e4m3_head_of(a.pages, row, has ? tile : tile0, kvh, in_page);
+    if (head < 0) head = 0;
     const uint8_t* at = a.pages.k + e4m3_tile_at(a.pages, head, in_page);
     const f32x4 scale = *reinterpret_cast<const f32x4*>(a.pages.k_scale + e4m3_scale_at(a.pages, head, in_page));
 #pragma unroll
@@ -771,65 +780,107 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DT > 8 ? 1 
         kf[jt][2 * i + 1] = numbers(w[2], w[3], scale[jt]);
       }
   }
-  // the tokens that may see a position of the tile: from the tile's first to the last whose reach has its last
-  const int from = max(pos0 - start, 0) / 16;
-  int to = n;
-  if (a.window > 0) to = (int)min((int64_t)to, (int64_t)pos0 + E4M3_TILE - 1 + a.window - start);
-  if (a.mod.chunk > 0) to = (int)min((int64_t)to, (int64_t)((pos0 + E4M3_TILE - 1) / a.mod.chunk + 1) * a.mod.chunk - start);
-  const int items = ((to + 15) / 16 - from) * g;
+  // the tokens that may see a position of the four tiles: from the first tile's first to the last whose reach has the last one's last
+  const int from = max(tile0 * E4M3_TILE - start, q_beg) / WEIGHT_TOKENS * WEIGHT_TOKENS, end_pos = (tile0 + 4) * E4M3_TILE - 1;
+  int to = q_end;
+  if (a.window > 0) to = (int)min((int64_t)to, (int64_t)end_pos + a.window - start);
+  if (a.mod.chunk > 0) to = (int)min((int64_t)to, (int64_t)(end_pos / a.mod.chunk + 1) * a.mod.chunk - start);
+  const int chunks = hd / PER;      // of 16 bytes in a row
+  u32x4 pq[CH];
+  float plse = 0.f;
+  auto ask = [&](int q0) {
+#pragma unroll
+    for (int j = 0; j < CH; ++j) {
+      const int i = min(tid + 256 * j, WEIGHT_TOKENS * chunks - 1);
+      pq[j] = *reinterpret_cast<const u32x4*>(a.q + ((int64_t)(t0 + min(q0 + i / chunks, n - 1)) * a.nh + h) * hd + i % chunks * PER);
+    }
+    if (tid < WEIGHT_TOKENS) plse = a.lse[(int64_t)(t0 + min(q0 + tid, n - 1)) * a.nh + h];
+  };
   f32x4 acc[4];
 #pragma unroll
   for (int jt = 0; jt < 4; ++jt) acc[jt] = f32x4{0.f, 0.f, 0.f, 0.f};
-  bf16x8 qf[KS][PIECES];
-  float lse;
-  auto ask = [&](int i) {
-    const int h = kvh * g + i % g, qi = (from + i / g) * 16 + r;
-    const int64_t at = (int64_t)(t0 + min(qi, n - 1)) * a.nh + h;
-    lse = a.lse[at];
+  if (from < to) ask(from);
+  int buf = 0;
+  for (int q0 = from; q0 < to; q0 += WEIGHT_TOKENS, buf ^= 1) {
+    // (one barrier a round: the buffer that is written was last read before the one before)
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) load_query(qf[ks], a.q + at * hd, 64 * (ks / 2) + 16 * c + 8 * (ks % 2), hd, true);
-  };
-  if (wave < items) ask(wave);
-  for (int i = wave; i < items; i += 4) {
-    const int h = kvh * g + i % g, q0 = (from + i / g) * 16, qi = q0 + r;
-    const int p = qi < n ? start + qi : -1, lo = reach_lo(p, a.window, a.mod.chunk);
-    const float r1 = MOD && a.mod.r1 ? a.mod.r1[h] : 0.f, r2 = MOD && a.mod.r1 ? a.mod.r2[h] : 0.f;
-    f32x4 s[4];
+    for (int j = 0; j < CH; ++j) {
+      const int i = min(tid + 256 * j, WEIGHT_TOKENS * chunks - 1);
+      *reinterpret_cast<u32x4*>(qs + (buf * WEIGHT_TOKENS + i / chunks) * PITCH + i % chunks * PER) = pq[j];
+    }
+    if (tid < WEIGHT_TOKENS) lses[buf][tid] = plse;
+    __syncthreads();
+    if (q0 + WEIGHT_TOKENS < to) ask(q0 + WEIGHT_TOKENS);
+    if (!has) continue;
 #pragma unroll
-    for (int jt = 0; jt < 4; ++jt) s[jt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int half = 0; half < 2; ++half) {
+      const int q1 = q0 + 16 * half, qi = q1 + r;
+      // some of the 16 tokens sees some of the tile
+      if (q1 >= n || start + min(q1 + 15, n - 1) < pos0 || reach_lo(start + q1, a.window, a.mod.chunk) >= pos0 + E4M3_TILE) continue;
+      const int p = qi < n ? start + qi : -1, lo = reach_lo(p, a.window, a.mod.chunk);
+      const act_t* qrow = qs + (buf * WEIGHT_TOKENS + 16 * half + r) * PITCH;
+      f32x4 s[4];
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks)
+      for (int jt = 0; jt < 4; ++jt) s[jt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        bf16x8 qf[PIECES];
+        load_query(qf, qrow, 64 * (ks / 2) + 16 * c + 8 * (ks % 2), hd, true);
+#pragma unroll
+        for (int jt = 0; jt < 4; ++jt)
+#pragma unroll
+          for (int pc = PIECES - 1; pc >= 0; --pc) s[jt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[jt][ks], qf[pc], s[jt], 0, 0, 0);
+      }
+      const float sum = lses[buf][16 * half + r];
+      // every token of the 16 sees the whole tile: nothing to compare
+      const bool masked = q1 + 15 >= n || start + q1 < pos0 + E4M3_TILE - 1 || reach_lo(start + q1 + 15, a.window, a.mod.chunk) > pos0;
+      final_scores<MOD>(s, a, ch, r1, r2, pos0, p, lo, masked);
 #pragma unroll
       for (int jt = 0; jt < 4; ++jt)
 #pragma unroll
-        for (int pc = PIECES - 1; pc >= 0; --pc) s[jt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[jt][ks], qf[ks][pc], s[jt], 0, 0, 0);
-    const float sum = lse;
-    if (i + 4 < items) ask(i + 4);      // (the next queries travel during the powers)
-    // every token of the 16 sees the whole tile: nothing to compare
-    const bool masked = q0 + 15 >= n || start + q0 < pos0 + E4M3_TILE - 1 || reach_lo(start + q0 + 15, a.window, a.mod.chunk) > pos0;
-    final_scores<MOD>(s, a, ch, r1, r2, pos0, p, lo, masked);
-#pragma unroll
-    for (int jt = 0; jt < 4; ++jt)
-#pragma unroll
-      for (int v = 0; v < 4; ++v) acc[jt][v] += __builtin_amdgcn_exp2f(fmaf(s[jt][v], MOD ? 1.f : ch.scale2, -sum));
-  }
-#pragma unroll
-  for (int jt = 0; jt < 4; ++jt)
-#pragma unroll
-    for (int v = 0; v < 4; ++v) {
-      const float x = lanes_fold<16>(acc[jt][v], LanesSum());
-      if (r == 0) sums[wave][16 * jt + 4 * c + v] = x;
+        for (int v = 0; v < 4; ++v) acc[jt][v] += __builtin_amdgcn_exp2f(fmaf(s[jt][v], MOD ? 1.f : ch.scale2, -sum));
     }
-  __syncthreads();
-  if (tid < E4M3_TILE && pos0 + tid < start + n) {
-    a.pages.weight[head * a.pages.page_size + in_page * E4M3_TILE + tid] += (sums[0][tid] + sums[1][tid]) + (sums[2][tid] + sums[3][tid]);
   }
+  if (!has) return;
+  float* out = a.scores + ((int64_t)blockIdx.z * a.nh + h) * a.ld_scores + pos0;
+#pragma unroll
+  for (int jt = 0; jt < 4; ++jt) {
+    f32x4 x;
+#pragma unroll
+    for (int v = 0; v < 4; ++v) x[v] = lanes_fold<16>(acc[jt][v], LanesSum());
+    if (r == 0) *reinterpret_cast<f32x4*>(out + 16 * jt + 4 * c) = x;
+  }
+}
+// grid (blocks of 1,024 positions, nkv, B): a thread adds what four neighbouring positions have received.
+__global__ __launch_bounds__(256) void e4m3_add_weights_kernel(E4m3Attn a, int cuts) {
+  const int kvh = blockIdx.y, b = blockIdx.z, g = a.nh / a.nkv, j = (int)blockIdx.x * 1024 + 4 * (int)threadIdx.x;
+  const int n = a.cu[b + 1] - a.cu[b], start = a.start[b], lo = reach_lo(start, a.window, a.mod.chunk);
+  if (n <= 0 || j >= start + n || j + 3 < lo) return;
+  int in_page;
+  const int64_t head = e4m3_head_of(a.pages, a.pages.table + (int64_t)a.slots[b] * a.pages.bt_stride, j / E4M3_TILE, kvh, in_page);
+  if (head < 0) return;
+  f32x4* to = reinterpret_cast<f32x4*>(a.pages.weight + head * a.pages.page_size + in_page * E4M3_TILE + j % E4M3_TILE);
+  f32x4 w = {0.f, 0.f, 0.f, 0.f};
+  for (int i = 0; i < cuts; ++i) {
+    const float* from = a.scores + (((int64_t)b * cuts + i) * a.nh + kvh * g) * a.ld_scores + j;
+#pragma unroll 4
+    for (int h = 0; h < g; ++h) w += *reinterpret_cast<const f32x4*>(from + h * a.ld_scores);
+  }
+  f32x4 was = *to;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) was[e] = j + e >= lo && j + e < start + n ? was[e] + w[e] : was[e];
+  *to = was;
 }
 
 // ------------------------------------------------------------------------------------------ launch
 // Waves of a step beyond which a wave takes more runs instead: two rounds of three waves to a SIMD.  us of the runs of 8 sequences of 8,192 tokens (16
 // heads) and of 64 of 300 to 4,100 (28 heads on 4): with 2,048 waves 52 and 55, 3,072 53 and 51, 4,096 59 and 51, 6,144 52 and 42, 8,192 55 and 42.
 #define DECODE_WAVES 6144
+// Cuts of a prompt's tokens for the columns' sums: as many as make some thousands of workgroups, of 256 tokens at least.
+static int e4m3_cuts(int B, int nh, int max_new, int max_end) {
+  const int64_t groups = (int64_t)((max_end + 4 * E4M3_TILE - 1) / (4 * E4M3_TILE)) * nh * B;
+  return (int)max((int64_t)1, min((int64_t)(max_new + 255) / 256, 4096 / groups));
+}
 template <int DT, bool MOD>
 static int launch_decode(const E4m3Attn& a, int max_end, hipStream_t st) {
   const int g = a.nh / a.nkv, columns = a.nkv * ((g + 15) / 16);
@@ -862,17 +913,29 @@ static int launch_prompt(const E4m3Attn& a, int max_new, hipStream_t st) {
 template <int DT, bool MOD>
 static int launch_as(const E4m3Attn& a, int decode, int max_new, int max_end, hipStream_t st) {
   if (decode) return launch_decode<DT, MOD>(a, max_end, st);
-  // two groups of 16 tokens to a wave halve the reads from LDS, where that leaves the chip a workgroup to a compute unit
+  // Two groups of 16 tokens to a wave halve the reads from LDS, and the chip does 733 TFLOP/s instead of 505 (8,192 tokens of 16 heads of
+  // 128), but it takes enough workgroups that the last blocks, which see most, do not stand alone: 2,048 tokens, 256 of
+  // them, take 47 us so and 42 with one group; 4,096 tokens, 512 of them, 101 and 136.
   constexpr int TWO = PIECES == 1 && DT <= 8 ? 2 : 1, HALVES = DT <= 8 ? 2 : 1;
-  const char* e1 = getenv("TQ_T1"); const char* e2 = getenv("TQ_T2");
-  const int64_t of_two = (int64_t)((max_new + 127) / 128) * a.nh * a.B;
-  int rc;
-  const bool two = TWO == 2 && of_two >= (e1 ? atoi(e1) : 192), halves = (TWO == 2 && two ? of_two : (int64_t)((max_new + 63) / 64) * a.nh * a.B) <= (e2 ? atoi(e2) : 512);
-  if (two) rc = halves ? launch_prompt<DT, TWO, MOD, HALVES>(a, max_new, st) : launch_prompt<DT, TWO, MOD, 1>(a, max_new, st);
-  else rc = halves ? launch_prompt<DT, 1, MOD, HALVES>(a, max_new, st) : launch_prompt<DT, 1, MOD, 1>(a, max_new, st);
-  if (rc) return rc;
-  if (a.lse)
-    hipLaunchKernelGGL((e4m3_prompt_weights_kernel<DT, MOD>), dim3((max_end + E4M3_TILE - 1) / E4M3_TILE, a.nkv, a.B), dim3(256), 0, st, a);
+  const int64_t of_two = (int64_t)((max_new + 127) / 128) * a.nh * a.B, of_one = (int64_t)((max_new + 63) / 64) * a.nh * a.B;
+  const bool two = TWO == 2 && of_two > 256;
+  // Tiles by turns in two halves of a workgroup: with few workgroups (4,096 tokens of 16 heads 134 -> 101 us, 2,048 of them 50 -> 42,
+  // 1,024 25 -> 19); with 1,536 of them 193 -> 232.
+  // Blocks behind a short window have no tiles to share (tokens of a 32-bit prompt behind 256 positions: 18 -> 20 us).
+  const int seen = a.window > 0 ? min(max_end, a.window + 64) : max_end;
+  const bool halves = HALVES == 2 && (two ? of_two : of_one) <= 512 && seen >= 8 * E4M3_TILE;
+  const int rc = two ? (halves ? launch_prompt<DT, TWO, MOD, HALVES>(a, max_new, st) : launch_prompt<DT, TWO, MOD, 1>(a, max_new, st))
+                     : (halves ? launch_prompt<DT, 1, MOD, HALVES>(a, max_new, st) : launch_prompt<DT, 1, MOD, 1>(a, max_new, st));
+  if (rc || !a.lse) return rc;
+  const int tiles = (max_end + E4M3_TILE - 1) / E4M3_TILE, cuts = e4m3_cuts(a.B, a.nh, max_new, max_end), cut = ((max_new + cuts - 1) / cuts + WEIGHT_TOKENS - 1) / WEIGHT_TOKENS * WEIGHT_TOKENS;
+  if ((int64_t)a.B * cuts > 65535) return TQ_ERR_UNSUPPORTED;
+  const size_t shmem = 2 * (size_t)WEIGHT_TOKENS * (16 * DT * sizeof(act_t) + 16);      // at most 65.5 KiB
+  if (shmem > 64 * 1024) {
+    const hipError_t e = hipFuncSetAttribute((const void*)e4m3_prompt_weights_kernel<DT, MOD>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)shmem);
+    if (e != hipSuccess) return (int)e;
+  }
+  hipLaunchKernelGGL((e4m3_prompt_weights_kernel<DT, MOD>), dim3((tiles + 3) / 4, a.nh, a.B * cuts), dim3(256), shmem, st, a, cuts, cut);
+  hipLaunchKernelGGL(e4m3_add_weights_kernel, dim3((max_end + 1023) / 1024, a.nkv, a.B), dim3(256), 0, st, a, cuts);
   return 0;
 }
 template <int DT>
@@ -880,11 +943,11 @@ static int launch(const E4m3Attn& a, int decode, int max_new, int max_end, hipSt
   return a.mod.cap > 0.f || a.mod.r1 || !(a.scale > 0.f) ? launch_as<DT, true>(a, decode, max_new, max_end, st) : launch_as<DT, false>(a, decode, max_new, max_end, st);
 }
 
-// Floats of scratch: for decoding the runs' sums, with weights the scores too; for prompts with weights the rows' sums.
-TQ_API int64_t tq_e4m3_attention_scratch(int T, int B, int nh, int nkv, int hd, int max_end, int decode, int weights) {
-  const int64_t rows = weights ? (int64_t)T * nh : 0;
-  if (!decode) return rows;
+// Floats of scratch: for decoding the runs' sums, with weights the scores too; for prompts with weights the columns' and the rows' sums.
+// max_new: the longest run.
+TQ_API int64_t tq_e4m3_attention_scratch(int T, int B, int nh, int nkv, int hd, int max_new, int max_end, int decode, int weights) {
   const int64_t ld = (max_end + E4M3_TILE - 1) / E4M3_TILE * E4M3_TILE;
+  if (!decode) return weights ? (int64_t)B * e4m3_cuts(B, nh, max_new, max_end) * nh * ld + (int64_t)T * nh : 0;
   return (int64_t)B * nh * e4m3_most_runs(max_end, nh / nkv) * (hd + 2) + (weights ? (int64_t)B * nh * ld : 0);
 }
 
@@ -902,17 +965,13 @@ TQ_API int tq_e4m3_attention(const void* q, void* out, const int* cu, const int*
   E4m3Attn a{(const act_t*)q, (act_t*)out, cu, slots, start, B, nh, nkv, window, scale, ScoreMod{softcap, r1, r2, chunk, sink, nullptr, 0},
              nullptr, e4m3_most_runs(max_end, nh / nkv), nullptr, 0, nullptr,
              E4m3Pages{(uint8_t*)k, (uint8_t*)v, (float*)k_scale, (float*)v_scale, weight, table, bt_stride, page_size, heads, head0, hd}};
-  if (decode) {
-    // (the scores first: their rows are read and written 16 bytes at a time)
-    if (weight) {
-      a.ld_scores = (max_end + E4M3_TILE - 1) / E4M3_TILE * E4M3_TILE;
-      a.scores = scratch;
-      scratch += (int64_t)B * nh * a.ld_scores;
-    }
-    a.partial = scratch;
-  } else if (weight) {
-    a.lse = scratch;
+  if (weight) {      // (first: its rows are read and written 16 bytes at a time)
+    a.ld_scores = (max_end + E4M3_TILE - 1) / E4M3_TILE * E4M3_TILE;
+    a.scores = scratch;
+    scratch += (decode ? (int64_t)B : (int64_t)B * e4m3_cuts(B, nh, max_new, max_end)) * nh * a.ld_scores;
+    if (!decode) a.lse = scratch;
   }
+  if (decode) a.partial = scratch;
   const int dt = hd / 16;
   const int rc = dt <= 4 ? launch<4>(a, decode, max_new, max_end, st) : dt <= 8 ? launch<8>(a, decode, max_new, max_end, st)
                : dt <= 12 ? launch<12>(a, decode, max_new, max_end, st) : launch<16>(a, decode, max_new, max_end, st);

@@ -171,7 +171,7 @@ _SIGNATURES = {
                        _c_ptr],
     "tq_e4m3_move": [_c_ptr, _c_ptr, _c_int, _c_ptr, _c_int, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int,
                      _c_int, _c_int, _c_ptr],
-    "tq_e4m3_attention_scratch": [_c_int] * 8,
+    "tq_e4m3_attention_scratch": [_c_int] * 9,
     "tq_e4m3_attention": [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_f32, _c_f32, _c_ptr,
                           _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_ptr,
                           _c_int, _c_int, _c_int, _c_ptr],
@@ -1507,7 +1507,7 @@ def attention_e4m3(q: torch.Tensor, pages: E4m3Pages, layer: int, num_heads: int
     where, B, max_new, max_end, decode = _e4m3_runs(k, runs, pages, T, dev)
     lib = library(act)
     out = torch.empty_like(q)
-    n = lib.tq_e4m3_attention_scratch(T, B, num_heads, nkv, hd, max_end, decode, add_weights) if decode or add_weights else 0
+    n = lib.tq_e4m3_attention_scratch(T, B, num_heads, nkv, hd, max_new, max_end, decode, add_weights) if decode or add_weights else 0
     scratch = torch.empty((n,), dtype=torch.float32, device=q.device) if n else None
     _run(k, lib.tq_e4m3_attention(
         q.data_ptr(), out.data_ptr(), *where, T, B, num_heads, nkv, hd, window or 0, scale, softcap or 0.0, _ptr(r1), _ptr(r2), chunk or 0,
