@@ -446,7 +446,7 @@ struct WeightOf {
 
 // Runs of all but the shortest sequences: grid (waves, nkv * ceil(g / 16), B), block 64; a wave streams through neighbouring runs.
 template <int DT, bool MOD>
-__global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(DT > 12 || DT * PIECES > 24 ? 1 : DT * PIECES > 8 ? 2 : 3))) void e4m3_decode_kernel(E4m3Attn a) {
+__global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(DT > 12 || DT * PIECES > 24 ? 1 : DT * PIECES >= 8 ? 2 : 3))) void e4m3_decode_kernel(E4m3Attn a) {
   const int b = blockIdx.z, g = a.nh / a.nkv, ngc = (g + 15) / 16;
   const int p = a.start[b], S = e4m3_tiles_per_run(p, g), lo = reach_lo(p, a.window, a.mod.chunk);
   const int first_run = lo / E4M3_TILE / S, n_runs = e4m3_runs_at(p, g) - first_run, each = (n_runs + (int)gridDim.x - 1) / (int)gridDim.x;
@@ -873,8 +873,9 @@ __global__ __launch_bounds__(256) void e4m3_add_weights_kernel(E4m3Attn a, int c
 }
 
 // ------------------------------------------------------------------------------------------ launch
-// Waves of a step beyond which a wave takes more runs instead: two rounds of three waves to a SIMD.  us of the runs of 8 sequences of 8,192 tokens (16
-// heads) and of 64 of 300 to 4,100 (28 heads on 4): with 2,048 waves 52 and 55, 3,072 53 and 51, 4,096 59 and 51, 6,144 52 and 42, 8,192 55 and 42.
+// Waves of a step beyond which a wave takes more runs instead: three rounds of two waves to a SIMD.  us of the runs of 8 sequences of 8,192 tokens (16
+// heads) and of 64 of 300 to 4,100 (28 heads on 4): with 2,048 waves 47 and 50, 3,072 52 and 46, 4,096 53 and 50, 6,144 47 and 41, 8,192 52 and
+// 41.  (Three waves to a SIMD, with some of their registers in scratch memory: 58 and 43 at best.)
 #define DECODE_WAVES 6144
 // Cuts of a prompt's tokens for the columns' sums: as many as make some thousands of workgroups, of 256 tokens at least.
 static int e4m3_cuts(int B, int nh, int max_new, int max_end) {

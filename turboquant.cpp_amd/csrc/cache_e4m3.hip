@@ -326,11 +326,27 @@ __device__ __forceinline__ uint32_t ordered(float w) {
   const uint32_t b = __float_as_uint(w == 0.f ? 0.f : w);      // (-0 equals 0)
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
+// Sums of all threads' numbers: of those in front of a thread, and of all.  `waves`: 16 words of LDS.
+__device__ __forceinline__ int sum_before(int v, int* waves, int& all) {
+  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  const int upto = wave_scan_add(v);
+  __syncthreads();
+  if (lane == 63) waves[wave] = upto;
+  __syncthreads();
+  int before = upto - v;
+  all = 0;
+#pragma unroll
+  for (int w = 0; w < 16; ++w) {
+    before += w < wave ? waves[w] : 0;
+    all += waves[w];
+  }
+  return before;
+}
 __global__ __launch_bounds__(1024) void e4m3_choice_kernel(E4m3Choice a) {
   extern __shared__ uint32_t held[];
-  __shared__ uint32_t hist[16][256];
+  __shared__ uint32_t hist[4][256];
   __shared__ int waves[16];
-  __shared__ uint32_t found[2];      // bytes found so far; how many of the bin are wanted
+  __shared__ uint32_t found[3];      // bytes found so far; how many of the bin are wanted; whether that is all of it
   const int head = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid % 64, wave = tid / 64;
   const int slot = a.slots[b];
   int* out = a.kept + ((int64_t)b * a.pages.heads + head) * a.keep;
@@ -351,33 +367,31 @@ __global__ __launch_bounds__(1024) void e4m3_choice_kernel(E4m3Choice a) {
   for (int j = lo + tid; j < in_lds; j += 1024) held[j - lo] = read(j);
   auto key = [&](int j) -> uint32_t { return j < in_lds ? held[j - lo] : read(j); };
   uint32_t prefix = 0u, want = m;
+  int shift = 24;
   if (m > 0) {
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      for (int i = tid; i < 16 * 256; i += 1024) hist[i / 256][i % 256] = 0u;
+    for (;; shift -= 8) {
+      hist[tid / 256][tid % 256] = 0u;
       __syncthreads();
       for (int j = lo + tid; j < hi; j += 1024) {
         const uint32_t k = key(j);
-        if (shift == 24 || (k >> (shift + 8)) == prefix) atomicAdd(&hist[wave][k >> shift & 255u], 1u);
-      }
-      __syncthreads();
-      if (tid < 256) {
-        uint32_t s = 0u;
-#pragma unroll
-        for (int w = 0; w < 16; ++w) s += hist[w][tid];
-        hist[0][tid] = s;
+        if (shift == 24 || (k >> (shift + 8)) == prefix) atomicAdd(&hist[wave % 4][k >> shift & 255u], 1u);
       }
       __syncthreads();
       if (wave == 0) {
         // four bins to a lane, from the highest: lane l holds bins 255 - 4 l .. 252 - 4 l
         uint32_t c[4], mine = 0u;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) mine += c[i] = hist[0][255 - 4 * lane - i];
+        for (int i = 0; i < 4; ++i) {
+          const int bin = 255 - 4 * lane - i;
+          mine += c[i] = hist[0][bin] + hist[1][bin] + hist[2][bin] + hist[3][bin];
+        }
         uint32_t above = (uint32_t)wave_scan_add((int)mine) - mine;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           if (above < want && above + c[i] >= want) {      // one bin alone
             found[0] = prefix << 8 | (uint32_t)(255 - 4 * lane - i);
             found[1] = want - above;
+            found[2] = above + c[i] == want;
           }
           above += c[i];
         }
@@ -385,40 +399,32 @@ __global__ __launch_bounds__(1024) void e4m3_choice_kernel(E4m3Choice a) {
       __syncthreads();
       prefix = found[0];
       want = found[1];
+      if (shift == 0 || found[2]) break;      // (a bin that stays whole needs no more bytes)
     }
   }
-  // prefix is the m-th largest weight, and the `want` first positions with that weight stay
-  int at = 0;      // kept so far
-  uint32_t same = 0u;      // of them and those left out, positions with that weight
-  for (int j0 = 0; j0 < n; j0 += 1024) {
-    const int j = j0 + tid;
-    const bool between = j >= lo && j < hi;
-    const uint32_t k = between && m > 0 ? key(j) : 0u;
-    const bool equal = between && m > 0 && k == prefix;
-    const uint64_t eq = __ballot(equal);
-    if (lane == 0) waves[wave] = __popcll(eq);
-    __syncthreads();
-    uint32_t before = same, all = 0u;
-    for (int w = 0; w < 16; ++w) {
-      before += w < wave ? waves[w] : 0;
-      all += waves[w];
+  // prefix is what the m-th largest weight's bytes from `shift` on are: larger ones stay, and of those with these bytes the `want` first.
+  // A thread takes neighbouring positions, so that two sums over threads place them all.
+  const int each = (n + 1023) / 1024, j0 = tid * each, j1 = min(j0 + each, n);
+  int equal = 0, stay = 0, all;
+  for (int j = j0; j < j1; ++j) {
+    if (j < lo || j >= hi) ++stay;
+    else if (m > 0) {
+      const uint32_t k = key(j) >> shift;
+      equal += k == prefix;
+      stay += k > prefix;
     }
-    before += __popcll(eq & ((1ull << lane) - 1ull));
-    same += all;
-    const bool stays = j < n && (!between || (m > 0 && (k > prefix || (equal && before < want))));
-    const uint64_t st = __ballot(stays);
-    __syncthreads();
-    if (lane == 0) waves[wave] = __popcll(st);
-    __syncthreads();
-    int to = at, total = 0;
-    for (int w = 0; w < 16; ++w) {
-      to += w < wave ? waves[w] : 0;
-      total += waves[w];
+  }
+  const int equal_before = sum_before(equal, waves, all);
+  int left = max((int)want - equal_before, 0);
+  if (m == 0) left = 0;
+  int to = sum_before(stay + min(left, equal), waves, all);
+  for (int j = j0; j < j1; ++j) {
+    bool s = j < lo || j >= hi;
+    if (!s && m > 0) {
+      const uint32_t k = key(j) >> shift;
+      s = k > prefix || (k == prefix && left-- > 0);
     }
-    to += __popcll(st & ((1ull << lane) - 1ull));
-    if (stays && to < a.keep) out[to] = j;
-    at += total;
-    __syncthreads();
+    if (s && to < a.keep) out[to++] = j;
   }
 }
 
@@ -442,9 +448,14 @@ TQ_API int tq_e4m3_choose(const int* slots, const int* lengths, int B, int max_l
 
 // ------------------------------------------------------------------------------------------ eviction: the move
 // A workgroup fills one tile of 64 positions of one sequence, layer and kv head from the positions that were chosen, each wherever it
-// lies: keys 16 bytes at a time, values, whose positions lie side by side, by bytes out of the source's tiles, which pass through LDS
-// one after the other (positions are in ascending order).  A block's scale is the largest of its positions' blocks; the codes
-// of the others are brought to it.  Rows behind the last position are zeros up to the end of their page.
+// lies: keys 16 bytes at a time; values, whose positions lie side by side, by bytes out of the source's tiles, which come through LDS whole,
+// three at a time (positions are in ascending order: a tile of which half the positions stay comes from two or three).  A thread
+// puts 16 positions of a dimension together.  A block's scale is the largest of its positions' blocks; the codes of the others are
+// brought to it.  Rows behind the last position are zeros up to the end of their page.
+// Bound by the bytes: lines of the source are read whole, twice what stays where every other position does.
+#define MOVE_TILES 3
+#define MOVE_PITCH 80      // bytes between the dimensions of a tile in LDS: 16 of them, four positions each, touch banks of their own
+typedef unsigned int u32x4_t __attribute__((ext_vector_type(4)));
 struct E4m3Move {
   const int* src;
   const int* dst;
@@ -452,10 +463,12 @@ struct E4m3Move {
   int keep, slots_of_table;
   E4m3Pages pages;
 };
+template <int VI>
 __global__ __launch_bounds__(256) void e4m3_move_kernel(E4m3Move a) {
-  extern __shared__ __attribute__((aligned(16))) uint8_t tiles[];      // two of [hd][68]: the source's values, the destination's
-  __shared__ int from[E4M3_TILE];
+  extern __shared__ __attribute__((aligned(16))) uint8_t tiles[];      // [3][hd][80]
+  __shared__ int from[E4M3_TILE], at_slot[E4M3_TILE], n_slots;      // places in the source; which of its tiles (numbered as they come)
   __shared__ int64_t head_of[E4M3_TILE];
+  __shared__ int64_t tile_of[E4M3_TILE];      // where the numbered tiles lie
   __shared__ float scale[2][E4M3_TILE], ratio[2][E4M3_TILE];
   const int hd = a.pages.hd, tid = threadIdx.x, b = blockIdx.z, head = blockIdx.y, tile = blockIdx.x, per = a.pages.page_size / E4M3_TILE;
   const int s = a.src[b], t = a.dst[b];
@@ -468,17 +481,22 @@ __global__ __launch_bounds__(256) void e4m3_move_kernel(E4m3Move a) {
   if (tid < E4M3_TILE) {
     const int i = tile * E4M3_TILE + tid;
     int j = i < a.keep ? a.kept[((int64_t)b * a.pages.heads + head) * a.keep + i] : -1;
-    if (j >= 0 && (j >= a.pages.bt_stride * a.pages.page_size || row[j / a.pages.page_size] < 0)) j = -1;
-    from[tid] = j;
-    const int64_t h = j < 0 ? 0 : (int64_t)row[j / a.pages.page_size] * a.pages.heads + head;
-    head_of[tid] = h;
+    int page = j >= 0 && j / a.pages.page_size < a.pages.bt_stride ? row[j / a.pages.page_size] : -1;
+    if (page < 0) j = -1;
+    const int64_t h = j < 0 ? 0 : (int64_t)page * a.pages.heads + head;
     const int64_t at = h * a.pages.page_size + (j < 0 ? 0 : j % a.pages.page_size);
     scale[0][tid] = j < 0 ? 0.f : a.pages.k_scale[at / E4M3_BLOCK];
     scale[1][tid] = j < 0 ? 0.f : a.pages.v_scale[at / E4M3_BLOCK];
     if (a.pages.weight) a.pages.weight[to * a.pages.page_size + in_page * E4M3_TILE + tid] = j < 0 ? 0.f : a.pages.weight[at];
+    from[tid] = j;
+    head_of[tid] = h;
+    const int mine = j < 0 ? -1 : j / E4M3_TILE, before = __shfl_up(mine, 1);
+    const uint64_t begins = __ballot(mine >= 0 && (tid == 0 || mine != before));
+    const int slot = __popcll(begins & (~0ull >> (63 - tid))) - 1;
+    at_slot[tid] = j < 0 ? -1 : slot;
+    if (begins >> tid & 1ull) tile_of[slot] = e4m3_tile_at(a.pages, h, j % a.pages.page_size / E4M3_TILE);
+    if (tid == 0) n_slots = __popcll(begins);
   }
-  uint8_t* mine = tiles + hd * 68;
-  for (int i = tid; i < hd * 17; i += 256) reinterpret_cast<uint32_t*>(mine)[i] = 0u;
   __syncthreads();
   if (tid < 2 * E4M3_TILE) {
     const int m = tid / E4M3_TILE, i = tid % E4M3_TILE;
@@ -487,43 +505,67 @@ __global__ __launch_bounds__(256) void e4m3_move_kernel(E4m3Move a) {
     ratio[m][i] = scale[m][i] * e4m3_inverse(top);
     if (i % E4M3_BLOCK == 0) (m ? a.pages.v_scale : a.pages.k_scale)[e4m3_scale_at(a.pages, to, in_page) + i / E4M3_BLOCK] = top;
   }
+  // keys on their way
+  u32x4_t keys[2 * VI];
+#pragma unroll
+  for (int i = 0; i < 2 * VI; ++i) {
+    const int at = tid + 256 * i, r = at % E4M3_TILE, ch = at / E4M3_TILE, j = from[r];
+    keys[i] = u32x4_t{0u, 0u, 0u, 0u};
+    if (ch < hd / 16 && j >= 0)
+      keys[i] = *reinterpret_cast<const u32x4_t*>(a.pages.k + e4m3_tile_at(a.pages, head_of[r], j % a.pages.page_size / E4M3_TILE) +
+                                                  ch * 16 * E4M3_TILE + j % E4M3_TILE * 16);
+  }
+  // this thread's 16 positions (of quarter c) in the source
+  const int c = tid % 4;
+  int off[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int p = 16 * (i / 4) + 4 * c + i % 4, q = from[p] % E4M3_TILE;
+    off[i] = from[p] < 0 ? -1 : at_slot[p] * (hd * MOVE_PITCH) + q % 16 / 4 * 16 + q / 16 * 4 + q % 4;
+  }
+  uint32_t w[2 * VI][4] = {};
+  const int slots = n_slots;
+  for (int s0 = 0; s0 < slots; s0 += MOVE_TILES) {
+    const int n = min(MOVE_TILES, slots - s0);
+    if (s0) __syncthreads();
+    for (int i = tid; i < n * hd * 4; i += 256)
+      *reinterpret_cast<u32x4_t*>(tiles + i / 4 * MOVE_PITCH + i % 4 * 16) =
+          *reinterpret_cast<const u32x4_t*>(a.pages.v + tile_of[s0 + i / (hd * 4)] + i % (hd * 4) * 16);
+    __syncthreads();
+    const int lo = s0 * (hd * MOVE_PITCH), hi = lo + n * (hd * MOVE_PITCH);
+#pragma unroll
+    for (int k = 0; k < 2 * VI; ++k) {
+      const int d = tid / 4 + 64 * k;
+      if (d < hd)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (off[i] >= lo && off[i] < hi) w[k][i / 4] |= (uint32_t)tiles[off[i] - lo + d * MOVE_PITCH] << 8 * (i % 4);
+    }
+  }
   __syncthreads();
   uint8_t* kt = a.pages.k + e4m3_tile_at(a.pages, to, in_page);
-  for (int i = tid; i < E4M3_TILE * (hd / 16); i += 256) {
-    const int r = i % E4M3_TILE, ch = i / E4M3_TILE, j = from[r];
-    uint4 w = make_uint4(0u, 0u, 0u, 0u);
-    if (j >= 0) {
-      w = *reinterpret_cast<const uint4*>(a.pages.k + e4m3_tile_at(a.pages, head_of[r], j % a.pages.page_size / E4M3_TILE) +
-                                          ch * 16 * E4M3_TILE + j % E4M3_TILE * 16);
-      const float f = ratio[0][r];
-      if (f != 1.f)
-        w = make_uint4(e4m3_rescale(w.x, f, f, f, f), e4m3_rescale(w.y, f, f, f, f), e4m3_rescale(w.z, f, f, f, f), e4m3_rescale(w.w, f, f, f, f));
-    }
-    *reinterpret_cast<uint4*>(kt + ch * 16 * E4M3_TILE + r * 16) = w;
+#pragma unroll
+  for (int i = 0; i < 2 * VI; ++i) {
+    const int at = tid + 256 * i, r = at % E4M3_TILE, ch = at / E4M3_TILE;
+    if (ch >= hd / 16) break;
+    const float f = ratio[0][r];
+    if (f != 1.f)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) keys[i][e] = e4m3_rescale(keys[i][e], f, f, f, f);
+    *reinterpret_cast<u32x4_t*>(kt + ch * 16 * E4M3_TILE + r * 16) = keys[i];
   }
-  // values: runs of destination rows that come from one tile of the source (the same for all threads)
-  for (int r = 0; r < E4M3_TILE;) {
-    const int j = from[r];
-    if (j < 0) {
-      ++r;
-      continue;
+  uint8_t* vt = a.pages.v + e4m3_tile_at(a.pages, to, in_page);
+#pragma unroll
+  for (int k = 0; k < 2 * VI; ++k) {
+    const int d = tid / 4 + 64 * k;
+    if (d >= hd) break;
+    u32x4_t o;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float* f = ratio[1] + 16 * j + 4 * c;
+      o[j] = e4m3_rescale(w[k][j], f[0], f[1], f[2], f[3]);
     }
-    int end = r + 1;
-    while (end < E4M3_TILE && from[end] >= 0 && from[end] / E4M3_TILE == j / E4M3_TILE) ++end;
-    const uint32_t* vt = reinterpret_cast<const uint32_t*>(a.pages.v + e4m3_tile_at(a.pages, head_of[r], j % a.pages.page_size / E4M3_TILE));
-    for (int i = tid; i < hd * 16; i += 256) reinterpret_cast<uint32_t*>(tiles)[i / 16 * 17 + i % 16] = vt[i];
-    __syncthreads();
-    for (int i = tid; i < hd * (end - r); i += 256) {
-      const int d = i % hd, q = r + i / hd, p = from[q] % E4M3_TILE;
-      mine[d * 68 + q % 16 / 4 * 16 + q / 16 * 4 + q % 4] = tiles[d * 68 + p % 16 / 4 * 16 + p / 16 * 4 + p % 4];
-    }
-    __syncthreads();
-    r = end;
-  }
-  uint32_t* vt = reinterpret_cast<uint32_t*>(a.pages.v + e4m3_tile_at(a.pages, to, in_page));
-  for (int i = tid; i < hd * 16; i += 256) {
-    const int d = i / 16, c = i % 16 / 4, j = i % 4, p = 16 * j + 4 * c;
-    vt[i] = e4m3_rescale(reinterpret_cast<const uint32_t*>(mine)[d * 17 + i % 16], ratio[1][p], ratio[1][p + 1], ratio[1][p + 2], ratio[1][p + 3]);
+    *reinterpret_cast<u32x4_t*>(vt + d * E4M3_TILE + 16 * c) = o;
   }
 }
 
@@ -538,7 +580,9 @@ TQ_API int tq_e4m3_move(const int* src, const int* dst, int B, const int* kept, 
   E4m3Move a{src, dst, kept, keep, slots_of_table,
              E4m3Pages{(uint8_t*)k, (uint8_t*)v, k_scale, v_scale, weight, table, bt_stride, page_size, heads, 0, hd}};
   const int tiles = (keep + page_size - 1) / page_size * (page_size / E4M3_TILE);
-  hipLaunchKernelGGL(e4m3_move_kernel, dim3(tiles, heads, B), dim3(256), 2 * (size_t)hd * 68, st, a);
+  const size_t shmem = (size_t)MOVE_TILES * hd * MOVE_PITCH;      // at most 60 KiB
+  if (hd <= 128) hipLaunchKernelGGL(e4m3_move_kernel<1>, dim3(tiles, heads, B), dim3(256), shmem, st, a);
+  else hipLaunchKernelGGL(e4m3_move_kernel<2>, dim3(tiles, heads, B), dim3(256), shmem, st, a);
   TQ_LAUNCH_CHECK();
   return 0;
 }
