@@ -28,12 +28,14 @@ struct E4m3Write {
 __device__ __forceinline__ float bias_at(const E4m3Write& a, int i) {
   return a.bias_type == TQ_BF16 ? to_f32(((const bf16_t*)a.bias)[i]) : ((const float*)a.bias)[i];
 }
-// (numbers col .. col + 3 of a token whose row begins `at` numbers behind `base`: 32 bits of offset from an address that all lanes share)
-__device__ __forceinline__ float4 four_at(const E4m3Write& a, const float* base, uint32_t at, int col) {
-  float4 v = *reinterpret_cast<const float4*>(base + (at + (uint32_t)col));
-  if (a.bias) v = make_float4(v.x + bias_at(a, col), v.y + bias_at(a, col + 1), v.z + bias_at(a, col + 2), v.w + bias_at(a, col + 3));
-  return v;
+__device__ __forceinline__ float4 bias_four(const E4m3Write& a, int i) {
+  if (a.bias_type == TQ_F32) return *reinterpret_cast<const float4*>((const float*)a.bias + i);
+  const uint2 w = *reinterpret_cast<const uint2*>((const bf16_t*)a.bias + i);
+  return make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xffff0000u));
 }
+__device__ __forceinline__ float4 plus(float4 x, float4 y) { return make_float4(x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w); }
+// Numbers col .. col + 3 of a token whose row begins `at` numbers behind `base`: 32 bits of offset from an address that all lanes share.
+__device__ __forceinline__ float4 four_at(const float* base, uint32_t at, int col) { return *reinterpret_cast<const float4*>(base + (at + (uint32_t)col)); }
 // Sine and cosine of the exact product p * f (48 bits, which 64-bit numbers hold), in 64 bits: reduced to an eighth of a turn about the
 // nearest quarter, then the series of sine and cosine, whose first omitted terms are r^13 / 13! and r^12 / 12! (1e-10 and less).  In 32
 // bits the product alone would be off by 0.004 at position 100,000, and the keys' codes would differ from exact ones more often than
@@ -47,12 +49,31 @@ __device__ __forceinline__ float2 turn_of(int p, float f, float amp) {
   const double cs = q == 0 ? c : q == 1 ? -s : q == 2 ? -c : s, sn = q == 0 ? s : q == 1 ? c : q == 2 ? -s : -c;
   return make_float2(amp * (float)cs, amp * (float)sn);
 }
-// Four neighbouring numbers of a head from dimension d on, rotated; `turn`: the token's cosines and sines.  FOURS: four numbers rotate
-// alike (pairs by halves, a multiple of four of them, or neighbouring pairs, an even number of them).
+// Four neighbouring numbers of a head from dimension d on, rotated, in two steps: what is read, and what becomes of it (`turn`: the token's
+// cosines and sines).  FOURS: four numbers rotate alike (pairs by halves, a multiple of four of them, or neighbouring pairs, an even
+// number of them).
+struct Raw {
+  float4 x, y;      // the numbers, and with pairs by halves their partners
+};
+// (Nothing waits in here: all that a thread needs is asked for before the first of it is used.)
 template <bool FOURS>
-__device__ __forceinline__ float4 rotated(const E4m3Write& a, const float* base, uint32_t at, int col, int d, const float2* turn) {
+__device__ __forceinline__ int partner_of(const E4m3Write& a, int d) {
   const int n = a.rot / 2;
-  const float4 x = four_at(a, base, at, col + d);
+  return FOURS && a.pairing == 0 && d < 2 * n ? (d < n ? d + n : d - n) : d;
+}
+template <bool FOURS>
+__device__ __forceinline__ Raw read_four(const E4m3Write& a, const float* base, uint32_t at, int col, int d) {
+  return Raw{four_at(base, at, col + d), four_at(base, at, col + partner_of<FOURS>(a, d))};
+}
+template <bool FOURS>
+__device__ __forceinline__ void add_bias(const E4m3Write& a, Raw& w, int col, int d) {
+  w.x = plus(w.x, bias_four(a, col + d));
+  w.y = plus(w.y, bias_four(a, col + partner_of<FOURS>(a, d)));
+}
+template <bool FOURS>
+__device__ __forceinline__ float4 rotated(const E4m3Write& a, const Raw& w, const float* base, uint32_t at, int col, int d, const float2* turn) {
+  const int n = a.rot / 2;
+  const float4 x = w.x, y = w.y;
   if (d >= 2 * n) return x;
   if constexpr (FOURS) {
     if (a.pairing == 1) {
@@ -60,7 +81,6 @@ __device__ __forceinline__ float4 rotated(const E4m3Write& a, const float* base,
       return make_float4(x.x * t0.x - x.y * t0.y, x.x * t0.y + x.y * t0.x, x.z * t1.x - x.w * t1.y, x.z * t1.y + x.w * t1.x);
     }
     const bool low = d < n;
-    const float4 y = four_at(a, base, at, col + (low ? d + n : d - n));
     const float2* t = turn + (low ? d : d - n);
     const float2 t0 = t[0], t1 = t[1], t2 = t[2], t3 = t[3];
     const float f = low ? -1.f : 1.f;
@@ -73,9 +93,9 @@ __device__ __forceinline__ float4 rotated(const E4m3Write& a, const float* base,
     if (e < 2 * n) {
       const bool low = a.pairing == 0 ? e < n : e % 2 == 0;
       const int other = col + (a.pairing == 0 ? (low ? e + n : e - n) : e ^ 1);
-      const float y = base[at + (uint32_t)other] + (a.bias ? bias_at(a, other) : 0.f);
+      const float z = base[at + (uint32_t)other] + (a.bias ? bias_at(a, other) : 0.f);
       const float2 t = turn[a.pairing == 0 ? (low ? e : e - n) : e / 2];
-      o[j] = o[j] * t.x + (low ? -y : y) * t.y;
+      o[j] = o[j] * t.x + (low ? -z : z) * t.y;
     }
   }
   return make_float4(o[0], o[1], o[2], o[3]);
@@ -104,16 +124,34 @@ __global__ __launch_bounds__(WRITE_THREADS) __attribute__((amdgpu_waves_per_eu(K
     const int nt = min(a.q_tokens, a.T - t0), heads = min(a.q_heads, a.nh - h0);
     for (int i = tid; i < nt * n; i += WRITE_THREADS) turns[i] = turn_of(a.positions[t0 + i / n], a.inv_freq[i % n], a.amp);
     __syncthreads();
+    // four items of a thread are on their way at a time
     const int items = nt * heads * fours;
-    for (int i = tid; i < items; i += WRITE_THREADS) {
-      const int d = i % fours * 4, th = i / fours, h = h0 + th % heads, t = th / heads;
-      const float4 o = rotated<FOURS>(a, a.x + (int64_t)t0 * a.ld, (uint32_t)t * ld, h * hd, d, turns + t * n);
-      act_t* out = a.q + ((int64_t)(t0 + t) * a.nh + h) * hd + d;
+    const float* base = a.x + (int64_t)t0 * a.ld;
+    for (int i0 = tid; i0 < items; i0 += 4 * WRITE_THREADS) {
+      Raw raw[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int i = min(i0 + u * WRITE_THREADS, items - 1), d = i % fours * 4, th = i / fours;
+        raw[u] = read_four<FOURS>(a, base, (uint32_t)(th / heads) * ld, (h0 + th % heads) * hd, d);
+      }
+      if (a.bias)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int i = min(i0 + u * WRITE_THREADS, items - 1);
+          add_bias<FOURS>(a, raw[u], (h0 + i / fours % heads) * hd, i % fours * 4);
+        }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int i = i0 + u * WRITE_THREADS, d = i % fours * 4, th = i / fours, h = h0 + th % heads, t = th / heads;
+        if (i >= items) break;
+        const float4 o = rotated<FOURS>(a, raw[u], base, (uint32_t)t * ld, h * hd, d, turns + t * n);
+        act_t* out = a.q + ((int64_t)(t0 + t) * a.nh + h) * hd + d;
 #if defined(TQ_ACT_BF16)
-      *reinterpret_cast<uint2*>(out) = make_uint2(f32_to_bf16_pair(o.x, o.y), f32_to_bf16_pair(o.z, o.w));
+        *reinterpret_cast<uint2*>(out) = make_uint2(f32_to_bf16_pair(o.x, o.y), f32_to_bf16_pair(o.z, o.w));
 #else
-      *reinterpret_cast<float4*>(out) = o;
+        *reinterpret_cast<float4*>(out) = o;
 #endif
+      }
     }
     return;
   }
@@ -130,36 +168,67 @@ __global__ __launch_bounds__(WRITE_THREADS) __attribute__((amdgpu_waves_per_eu(K
   for (int i = tid; i < WRITE_HEADS * 8; i += WRITE_THREADS) top[i / 8][i / 4 % 2][i % 4] = 0u;
   if (tid < WRITE_HEADS * 2) bad[tid / 2][tid % 2] = 0u;
   const int64_t first = (int64_t)t0 + pos0 - start;      // packed row of the tile's row 0 (rows before r0 are not read)
+  const int lane = tid % 64;
+  const float* base = a.x + first * a.ld;
+  float v[VI][16];
+  // (rows that are not new, and places behind the last item, read what lies next: one address instead of a condition around every load)
+  auto ask_values = [&](int kvh) {
+    const int vcol = (a.nh + a.nkv + kvh) * hd;
+#pragma unroll
+    for (int i = 0; i < VI; ++i) {
+      const int at = tid + i * WRITE_THREADS, d = at % hd, c = min(at / hd, 3);
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const int r = min(max(16 * (j / 4) + 4 * c + j % 4, r0), r1 - 1);
+        v[i][j] = base[(uint32_t)r * ld + (uint32_t)(vcol + d)];
+      }
+    }
+  };
+  int in_page;
+  const int64_t head0 = e4m3_head_of(a.pages, a.pages.table + (int64_t)a.slots[b] * a.pages.bt_stride, tile, kvh0, in_page);
+  if (head0 < 0) return;
+  ask_values(kvh0);      // (on their way while the angles are worked out)
   for (int i = tid; i < (r1 - r0) * n; i += WRITE_THREADS)
     turns[i] = turn_of(a.positions[first + r0 + i / n], a.inv_freq[i % n], a.amp);
   __syncthreads();
-  const int lane = tid % 64;
-  const float* base = a.x + first * a.ld;
 #pragma unroll 1
   for (int hi = 0; hi < a.kv_heads && kvh0 + hi < a.nkv; ++hi) {
     // (places are worked out anew for every head: kept, they would be more registers than a wave has)
     asm volatile("" : "+v"(tid));
-    const int kvh = kvh0 + hi;
-    int in_page;
-    const int64_t head = e4m3_head_of(a.pages, a.pages.table + (int64_t)a.slots[b] * a.pages.bt_stride, tile, kvh, in_page);
-    if (head < 0) return;      // (the same for every head of the tile)
-    const int kcol = (a.nh + kvh) * hd, vcol = (a.nh + a.nkv + kvh) * hd;
+    const int kvh = kvh0 + hi, kcol = (a.nh + kvh) * hd;
+    const int64_t head = head0 + hi;
     float4 k[KI];
-    float v[VI][16];
+    {
+      Raw raw[KI];
 #pragma unroll
-    for (int i = 0; i < KI; ++i) {
-      const int at = tid + i * WRITE_THREADS, r = at / fours;
-      k[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (r >= r0 && r < r1) k[i] = rotated<FOURS>(a, base, (uint32_t)r * ld, kcol, at % fours * 4, turns + (r - r0) * n);
-    }
+      for (int i = 0; i < KI; ++i) {
+        const int at = tid + i * WRITE_THREADS, r = min(max(at / fours, r0), r1 - 1);
+        raw[i] = read_four<FOURS>(a, base, (uint32_t)r * ld, kcol, at % fours * 4);
+      }
+      if (a.bias) {
 #pragma unroll
-    for (int i = 0; i < VI; ++i) {
-      const int at = tid + i * WRITE_THREADS, d = at % hd, c = at / hd;
-      const float add = a.bias && c < 4 ? bias_at(a, vcol + d) : 0.f;
+        for (int i = 0; i < KI; ++i) add_bias<FOURS>(a, raw[i], kcol, (tid + i * WRITE_THREADS) % fours * 4);
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        const int r = 16 * (j / 4) + 4 * c + j % 4;
-        v[i][j] = c < 4 && r >= r0 && r < r1 ? (base + (int64_t)(16 * (j / 4) + j % 4) * a.ld)[(uint32_t)(4 * c) * ld + (uint32_t)(vcol + d)] + add : 0.f;
+        for (int i = 0; i < VI; ++i) {
+          const float add = bias_at(a, kcol + a.nkv * hd + (tid + i * WRITE_THREADS) % hd);
+#pragma unroll
+          for (int j = 0; j < 16; ++j) v[i][j] += add;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < KI; ++i) {
+        const int at = tid + i * WRITE_THREADS, r = min(max(at / fours, r0), r1 - 1), d = at % fours * 4;
+        k[i] = rotated<FOURS>(a, raw[i], base, (uint32_t)r * ld, kcol, d, turns + (r - r0) * n);
+        if (at / fours != r) k[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+#pragma unroll
+      for (int i = 0; i < VI; ++i) {
+        const int c = (tid + i * WRITE_THREADS) / hd;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const int r = 16 * (j / 4) + 4 * c + j % 4;
+          if (c >= 4 || r < r0 || r >= r1) v[i][j] = 0.f;
+        }
       }
     }
     // largest magnitudes by block, and rows that are not finite
@@ -272,6 +341,7 @@ __global__ __launch_bounds__(WRITE_THREADS) __attribute__((amdgpu_waves_per_eu(K
       }
     }
     if (a.pages.weight && tid >= r0 && tid < r1) a.pages.weight[head * a.pages.page_size + in_page * E4M3_TILE + tid] = 0.f;
+    if (hi + 1 < a.kv_heads && kvh + 1 < a.nkv) ask_values(kvh + 1);
   }
 }
 
@@ -460,7 +530,7 @@ struct E4m3Move {
   const int* src;
   const int* dst;
   const int* kept;
-  int keep, slots_of_table;
+  int keep, slots_of_table, tiles;
   E4m3Pages pages;
 };
 template <int VI>
@@ -470,7 +540,10 @@ __global__ __launch_bounds__(256) void e4m3_move_kernel(E4m3Move a) {
   __shared__ int64_t head_of[E4M3_TILE];
   __shared__ int64_t tile_of[E4M3_TILE];      // where the numbered tiles lie
   __shared__ float scale[2][E4M3_TILE], ratio[2][E4M3_TILE];
-  const int hd = a.pages.hd, tid = threadIdx.x, b = blockIdx.z, head = blockIdx.y, tile = blockIdx.x, per = a.pages.page_size / E4M3_TILE;
+  // neighbouring tiles, which share lines of the source, on one die: workgroups are dealt to the eight dies by turns
+  const int64_t all = gridDim.x, at_once = all % 8 == 0 ? (int64_t)(blockIdx.x % 8) * (all / 8) + blockIdx.x / 8 : blockIdx.x;
+  const int tile = (int)(at_once % a.tiles), head = (int)(at_once / a.tiles % a.pages.heads), b = (int)(at_once / a.tiles / a.pages.heads);
+  const int hd = a.pages.hd, tid = threadIdx.x, per = a.pages.page_size / E4M3_TILE;
   const int s = a.src[b], t = a.dst[b];
   if (s < 0 || s >= a.slots_of_table || t < 0 || t >= a.slots_of_table) return;
   const int to_page = a.pages.table[(int64_t)t * a.pages.bt_stride + tile / per];
@@ -576,13 +649,14 @@ TQ_API int tq_e4m3_move(const int* src, const int* dst, int B, const int* kept, 
                         hipStream_t st) {
   if (B <= 0) return 0;
   if (keep < 1) return TQ_ERR_BAD_ARG;
-  if (!e4m3_pages_fit(page_size, heads, 0, 1, hd) || heads > 65535 || B > 65535 || keep > (int64_t)bt_stride * page_size) return TQ_ERR_UNSUPPORTED;
-  E4m3Move a{src, dst, kept, keep, slots_of_table,
+  if (!e4m3_pages_fit(page_size, heads, 0, 1, hd) || keep > (int64_t)bt_stride * page_size) return TQ_ERR_UNSUPPORTED;
+  E4m3Move a{src, dst, kept, keep, slots_of_table, (keep + page_size - 1) / page_size * (page_size / E4M3_TILE),
              E4m3Pages{(uint8_t*)k, (uint8_t*)v, k_scale, v_scale, weight, table, bt_stride, page_size, heads, 0, hd}};
-  const int tiles = (keep + page_size - 1) / page_size * (page_size / E4M3_TILE);
+  const int64_t groups = (int64_t)a.tiles * heads * B;
+  if (groups > 0xFFFFFF) return TQ_ERR_UNSUPPORTED;      // (a launch's threads are counted in 32 bits)
   const size_t shmem = (size_t)MOVE_TILES * hd * MOVE_PITCH;      // at most 60 KiB
-  if (hd <= 128) hipLaunchKernelGGL(e4m3_move_kernel<1>, dim3(tiles, heads, B), dim3(256), shmem, st, a);
-  else hipLaunchKernelGGL(e4m3_move_kernel<2>, dim3(tiles, heads, B), dim3(256), shmem, st, a);
+  if (hd <= 128) hipLaunchKernelGGL(e4m3_move_kernel<1>, dim3((unsigned)groups), dim3(256), shmem, st, a);
+  else hipLaunchKernelGGL(e4m3_move_kernel<2>, dim3((unsigned)groups), dim3(256), shmem, st, a);
   TQ_LAUNCH_CHECK();
   return 0;
 }

@@ -1372,30 +1372,33 @@ class E4m3Pages:
 
     def __post_init__(self):
         """Checks the pools once, for all calls with these pages."""
-        k, dev = "E4m3Pages", self.k.get_device()
-        shape = self.k.shape
-        _need(len(shape) == 4 and dev >= 0, k, "k must be [pages, layers, kv heads, page_size * head_dim] on the GPU")
+        k, table, w = self.k, self.table, self.weight
+        shape, dev, code = k.shape, k.get_device(), torch.float8_e4m3fn
+        ps = self.k_scale.shape[-1] * E4M3_BLOCK
+        hd = shape[-1] // ps if ps else 0
+        small, at = (*shape[:-1], ps // E4M3_BLOCK), table.shape
+        if not (dev >= 0 and len(shape) == 4 and ps % 64 == 0 and hd % 16 == 0 and 16 <= hd <= 256 and shape[3] == hd * ps and len(at) == 2
+                and _lies(k, code, shape, dev) and _lies(self.v, code, shape, dev) and _lies(self.k_scale, torch.float32, small, dev)
+                and _lies(self.v_scale, torch.float32, small, dev) and _lies(table, torch.int32, at, dev)
+                and (w is None or _lies(w, torch.float32, (*shape[:3], ps), dev)) and k.numel() and not (k.data_ptr() | self.v.data_ptr()) % 16):
+            self._explain()
+        self.__dict__.update(page_size=ps, head_dim=hd, layers=shape[1], num_kv_heads=shape[2], device_index=dev, table_shape=(at[0], at[1]))
+
+    def _explain(self):
+        k, shape = "E4m3Pages", self.k.shape
+        _need(len(shape) == 4 and self.k.is_cuda, k, "k must be [pages, layers, kv heads, page_size * head_dim] on the GPU")
         ps = self.k_scale.shape[-1] * E4M3_BLOCK
         _need(ps > 0 and ps % 64 == 0, k, lambda: f"pages must hold a multiple of 64 positions, hold {ps}")
         _need(shape[3] % (16 * ps) == 0 and 16 <= shape[3] // ps <= 256, k,
               lambda: f"a head of {shape[3] / ps:g} numbers is none of the multiples of 16 up to 256 that 8-bit pages take")
-        pools = [("k", self.k, torch.float8_e4m3fn, shape), ("v", self.v, torch.float8_e4m3fn, shape),
-                 ("k_scale", self.k_scale, torch.float32, (*shape[:3], ps // E4M3_BLOCK)),
-                 ("v_scale", self.v_scale, torch.float32, (*shape[:3], ps // E4M3_BLOCK))]
-        if self.weight is not None:
-            pools.append(("weight", self.weight, torch.float32, (*shape[:3], ps)))
-        for name, t, dtype, want in pools:
-            _check_here(t, k, name, dtype, want, dev)
-        _check_here(self.table, k, "table", torch.int32, None, dev)
+        dev, small = self.k.get_device(), (*shape[:3], ps // E4M3_BLOCK)
+        for name, t, dtype, want in (("k", self.k, torch.float8_e4m3fn, shape), ("v", self.v, torch.float8_e4m3fn, shape),
+                                     ("k_scale", self.k_scale, torch.float32, small), ("v_scale", self.v_scale, torch.float32, small),
+                                     ("weight", self.weight, torch.float32, (*shape[:3], ps)), ("table", self.table, torch.int32, None)):
+            if t is not None:
+                _check_here(t, k, name, dtype, want, dev)
         _need(self.table.dim() == 2, k, "table must be [slots, pages]")
-        _need(min(shape[:3]) >= 1 and self.k.data_ptr() % 16 == 0 and self.v.data_ptr() % 16 == 0, k, "pools must hold pages, from a multiple of 16 bytes on")
-        put = object.__setattr__
-        put(self, "page_size", ps)
-        put(self, "head_dim", shape[3] // ps)
-        put(self, "layers", shape[1])
-        put(self, "num_kv_heads", shape[2])
-        put(self, "device_index", dev)
-        put(self, "table_shape", tuple(self.table.shape))
+        raise KernelError(f"{k}: pools must hold pages, from a multiple of 16 bytes on")
 
     @classmethod
     def empty(cls, n_pages: int, layers: int, num_kv_heads: int, head_dim: int, page_size: int, table: torch.Tensor,
@@ -1419,6 +1422,11 @@ class E4m3Pages:
         return self.device_index
 
 
+def _lies(t: torch.Tensor, dtype, shape, device: int) -> bool:
+    """Whether it is a contiguous tensor of that type and shape on GPU ``device``."""
+    return isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and t.get_device() == device and t.is_contiguous()
+
+
 def _check_here(t: torch.Tensor, kernel: str, name: str, dtype, shape, device: int) -> None:
     """``_check`` and that the tensor lies on GPU ``device``, in as little of the host's time as a call that is right needs."""
     if not (isinstance(t, torch.Tensor) and t.dtype is dtype and (shape is None or t.shape == shape) and t.get_device() == device and t.is_contiguous()):
@@ -1429,14 +1437,16 @@ def _check_here(t: torch.Tensor, kernel: str, name: str, dtype, shape, device: i
 def _e4m3_runs(k: str, runs: dict, pages: E4m3Pages, T: int, dev: int):
     cu, slots, start = runs["cu_seqlens"], runs["slots"], runs["start"]
     B = slots.numel()
-    _check_here(cu, k, "cu_seqlens", torch.int32, (B + 1,), dev)
-    _check_here(slots, k, "slots", torch.int32, (B,), dev)
-    _check_here(start, k, "start", torch.int32, (B,), dev)
+    if not (_lies(cu, torch.int32, (B + 1,), dev) and _lies(slots, torch.int32, (B,), dev) and _lies(start, torch.int32, (B,), dev)):
+        _check_here(cu, k, "cu_seqlens", torch.int32, (B + 1,), dev)
+        _check_here(slots, k, "slots", torch.int32, (B,), dev)
+        _check_here(start, k, "start", torch.int32, (B,), dev)
     max_new, max_end, decode = int(runs["max_new"]), int(runs["max_end"]), bool(runs["decode"])
+    if 0 < max_end <= pages.table_shape[1] * pages.page_size and 1 <= max_new <= T and B <= T and (not decode or (T == B and max_new == 1)):
+        return (cu.data_ptr(), slots.data_ptr(), start.data_ptr()), B, max_new, max_end, decode
     _need(0 < max_end <= pages.table_shape[1] * pages.page_size, k, "positions reach beyond the page table")
     _need(1 <= max_new <= T and B <= T, k, "the runs do not fit the tokens")
-    _need(not decode or (T == B and max_new == 1), k, "decoding brings one token per sequence")
-    return (cu.data_ptr(), slots.data_ptr(), start.data_ptr()), B, max_new, max_end, decode
+    raise KernelError(f"{k}: decoding brings one token per sequence")
 
 
 def rope_kv_write_e4m3(qkv: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, pairing: int, rotary_dim: int,
