@@ -15,8 +15,8 @@ import numpy as np
 import torch
 
 from .csrc import ops
-from .cache.paged import CacheError
-from .engine.generate import GenerationOptions, GenerationResult, continue_in_slot, generate
+from .cache.paged import POOLS, CacheError
+from .engine.generate import GenerationOptions, GenerationResult, continue_in_slot, generate, kept_when_full
 from .engine.model import load_model, random_model
 from .engine.step import Engine
 
@@ -34,19 +34,25 @@ class Model:
     generated tokens) of a sequence, which the cache is sized for; a sequence that reaches it ends with reason
     ``"context"`` (0: the model's ``max_position_embeddings``, at most 4096 as in the reference,
     /root/reference/src/engine/tq_model.c:2951).  ``max_batch``: sequences that generate together.
+
+    ``kv_cache``: ``"same"`` (keys and values are cached in ``dtype``) or ``"e4m3"`` (in 8 bits, with a scale for every 16 positions,
+    by the layers that can read them: half the memory of 16 bits, or a quarter of 32).  ``when_full``: what happens to a sequence of
+    ``generate`` that reaches ``context_length``: ``"end"``, or ``"evict"``: half of its positions are let go, those that have received
+    little attention, and it goes on (with ``kv_cache="e4m3"``, for models whose layers all keep such a cache and see all of it; a
+    conversation does not let positions go).
     """
 
     def __init__(self, path: str, *, temperature: float = 0.7, top_p: float = 0.9, max_tokens: int = 256,
                  context_length: int = 0, dtype: str = "bfloat16", seed: int = 42, rep_penalty: float = 1.1,
                  max_batch: int = 8, device: str = "cuda:0", stop_tokens: Sequence[int] | None = None,
-                 f32_matrices: str = "bfloat16"):
+                 f32_matrices: str = "bfloat16", kv_cache: str = "same", when_full: str = "end"):
         """``f32_matrices``: with ``dtype="bfloat16"``, matrices that the folder stores in 32 bits are rounded to
         bfloat16 as they are loaded ("bfloat16"), or stay as they are stored ("keep": their products are slow)."""
         if not os.path.isdir(path):
             raise FileNotFoundError(f"model folder not found: {path}")
         self._path = path
         self._model = load_model(path, act=dtype, device=device, f32_matrices=f32_matrices)
-        self._setup(temperature, top_p, max_tokens, context_length, seed, rep_penalty, max_batch, stop_tokens)
+        self._setup(temperature, top_p, max_tokens, context_length, seed, rep_penalty, max_batch, stop_tokens, kv_cache, when_full)
 
     @classmethod
     def from_random(cls, config_json: dict, seed: int, **kw) -> "Model":
@@ -54,15 +60,19 @@ class Model:
         self = cls.__new__(cls)
         self._path = "<random>"
         opts = dict(temperature=0.7, top_p=0.9, max_tokens=256, context_length=0, dtype="bfloat16",
-                    gen_seed=42, rep_penalty=1.1, max_batch=8, device="cuda:0", stop_tokens=None, std=0.02, norm_std=0.0)
+                    gen_seed=42, rep_penalty=1.1, max_batch=8, device="cuda:0", stop_tokens=None, std=0.02, norm_std=0.0,
+                    kv_cache="same", when_full="end")
         opts.update(kw)
         self._model = random_model(config_json, seed, act=opts["dtype"], device=opts["device"], std=opts["std"],
                                    norm_std=opts["norm_std"])
         self._setup(opts["temperature"], opts["top_p"], opts["max_tokens"], opts["context_length"], opts["gen_seed"],
-                    opts["rep_penalty"], opts["max_batch"], opts["stop_tokens"])
+                    opts["rep_penalty"], opts["max_batch"], opts["stop_tokens"], opts["kv_cache"], opts["when_full"])
         return self
 
-    def _setup(self, temperature, top_p, max_tokens, context_length, seed, rep_penalty, max_batch, stop_tokens):
+    def _setup(self, temperature, top_p, max_tokens, context_length, seed, rep_penalty, max_batch, stop_tokens, kv_cache="same",
+               when_full="end"):
+        if when_full not in ("end", "evict"):
+            raise ValueError(f"when_full is 'end' or 'evict', got {when_full!r}")
         plan = self._model.plan
         ctx = context_length if context_length > 0 else min(plan.max_positions, 4096)
         ctx = min(ctx, plan.max_positions)
@@ -70,12 +80,17 @@ class Model:
         self._chat_slot, self._chat_tokens, self.last_finish_reason = None, [], None
         self.options = GenerationOptions(
             max_tokens=max_tokens, temperature=temperature, top_p=top_p, seed=seed, rep_penalty=rep_penalty,
-            stop_tokens=tuple(stop_tokens) if stop_tokens is not None else tuple(plan.stop_tokens), max_batch=max_batch)
+            stop_tokens=tuple(stop_tokens) if stop_tokens is not None else tuple(plan.stop_tokens), max_batch=max_batch,
+            when_full=when_full)
         page = 64
         per_seq = -(-ctx // page) * page
         # the cache holds ``max_batch`` sequences of ``context_length`` positions, and no sequence may grow beyond that
-        self._engine = Engine(self._model, max_tokens=per_seq * max_batch, page_size=page, max_slots=max_batch,
-                              max_positions=ctx)
+        # (and, where a full one lets positions go, what one of them keeps until its old pages are given back)
+        spare = -(-kept_when_full(ctx)[0] // page) * page if when_full == "evict" else 0
+        self._engine = Engine(self._model, max_tokens=per_seq * max_batch + spare, page_size=page, max_slots=max_batch,
+                              max_positions=ctx, kv_cache=kv_cache, track_weights=when_full == "evict")
+        if when_full == "evict" and self._engine.no_eviction() is not None:
+            raise ValueError(f"when_full='evict': {self._engine.no_eviction()}")
 
     # ------------------------------------------------------------ generation
     def generate(self, prompts, **overrides) -> list[list[int]]:
@@ -186,9 +201,10 @@ class Model:
         tensors = {"tokens": torch.tensor(self._chat_tokens[:data["length"]], dtype=torch.int32)}
         groups = []
         for i, g in enumerate(data["groups"]):
-            tensors[f"group.{i}.keys"] = g["keys"]
-            if g["values"] is not None:
-                tensors[f"group.{i}.values"] = g["values"]
+            for name in POOLS:
+                if g.get(name) is not None:      # (the file's types have none of 8 bits: codes go four to a word)
+                    t = g[name]
+                    tensors[f"group.{i}.{name}"] = t.view(torch.int32) if t.dtype == torch.uint8 else t
             groups.append({"first_page": g["first_page"], "entries": g["entries"], "key": list(g["key"])})
         for e, st in data["states"].items():
             tensors[f"state.{e}"] = st
@@ -210,9 +226,9 @@ class Model:
                 raise RuntimeError(f"{path} was saved by a {meta.get('dtype')} model, this one is {self._model.act}")
             groups = []
             for i, g in enumerate(json.loads(meta["groups"])):
-                values = f.read(f"group.{i}.values").clone() if f"group.{i}.values" in f.entries else None
-                groups.append({"first_page": g["first_page"], "entries": g["entries"], "key": tuple(g["key"]),
-                               "keys": f.read(f"group.{i}.keys").clone(), "values": values})
+                held = {n: f.read(f"group.{i}.{n}").clone() for n in POOLS if f"group.{i}.{n}" in f.entries}
+                held = {n: t.view(torch.uint8) if t.dtype == torch.int32 else t for n, t in held.items()}
+                groups.append({"first_page": g["first_page"], "entries": g["entries"], "key": tuple(g["key"]), "values": None, **held})
             states = {int(n.split(".")[1]): f.read(n).clone() for n in f.entries if n.startswith("state.")}
             tokens = f.read("tokens").tolist()
             data = {"length": int(meta["length"]), "page_size": int(meta["page_size"]), "groups": groups, "states": states}

@@ -23,6 +23,10 @@ blocks on demand with create / append / seq_len / free calls and status checks
   updated only when pages change hands; kernels find a token's rows through its slot.
 * A schedule entry that reads another entry's cache gets a view of that entry's storage and none
   of its own.
+* With ``kv_cache="e4m3"`` the groups whose mixers (and all that read their cache) can work on pages of 8 bits keep such
+  (``ops.E4m3Pages``); the others stay as they are.  If every group does, without windows and chunks, and keeps the attention
+  weight that each position receives (``track_weights``), positions can be let go: they are copied to other pages, and the sequence's
+  length is what is left, while its tokens' positions go on counting (``Slot.dropped`` is the difference).
 
 All bookkeeping is on the host and independent of the device, so it is tested without one.
 """
@@ -32,6 +36,10 @@ from dataclasses import dataclass, field
 
 import numpy as np
 import torch
+
+
+# what a group's pools hold (CacheGroup.pools), in the order in which a saved sequence lists them
+POOLS = ("keys", "values", "key_scales", "value_scales", "weights")
 
 
 class CacheError(RuntimeError):
@@ -78,6 +86,7 @@ class GroupKey:
     window: int | None
     chunk: int | None = None
     keep_first: int = 0
+    e4m3: bool = False
 
 
 @dataclass
@@ -94,11 +103,13 @@ class KVView:
     v_layer_offset: int = 0           # the same for values; equal to the keys' when both rows are as wide
     v_page_stride: int = 0
     value_dim: int = 0
+    pages8: "object | None" = None    # ops.E4m3Pages: the group keeps 8 bits, and k_pages and v_pages are None
+    layer: int = 0                    # the entry's layer in them
 
 
 class CacheGroup:
     def __init__(self, key: GroupKey, entries: list[int], n_pages: int, page_size: int, max_slots: int,
-                 max_pages_per_seq: int, dtype: torch.dtype, device):
+                 max_pages_per_seq: int, dtype: torch.dtype, device, track_weights: bool = False):
         self.key = key
         self.entries = entries
         self.page_size = page_size
@@ -108,18 +119,46 @@ class CacheGroup:
         self.v_page_stride = len(entries) * self.v_layer_elems
         self.pool = PagePool(n_pages)
         self.max_pages_per_seq = max_pages_per_seq
-        self.host_table = np.full((max_slots, max_pages_per_seq), -1, dtype=np.int32)
+        # (one row more where positions can be let go: the pages that they are copied to, before they become the sequence's)
+        self.spare = max_slots if key.e4m3 else None
+        rows = max_slots + (1 if key.e4m3 else 0)
+        self.host_table = np.full((rows, max_pages_per_seq), -1, dtype=np.int32)
         self.dirty: set[int] = set()
         self.device = device
         self._staging = None
-        self.k_pages = self.v_pages = self.table = None     # without a device: bookkeeping only
-        if device is not None:
+        self.k_pages = self.v_pages = self.table = self.pages8 = None     # without a device: bookkeeping only
+        if device is not None and key.e4m3:
+            if torch.device(device).type != "cuda":
+                raise CacheError("a cache of 8 bits lies on a GPU")
+            from ..csrc import ops
+            self.table = torch.full((rows, max_pages_per_seq), -1, dtype=torch.int32, device=device)
+            self.pages8 = ops.E4m3Pages.empty(n_pages, len(entries), key.num_kv_heads, key.head_dim, page_size, self.table, track_weights)
+        elif device is not None:
             # zeroed once: rows beyond a sequence's length are read by tiled kernels (and masked), so they
             # must always hold finite numbers; pages that come back from a sequence do
             self.k_pages = torch.zeros(n_pages * self.page_stride, dtype=dtype, device=device)
             if self.v_page_stride:
                 self.v_pages = torch.zeros(n_pages * self.v_page_stride, dtype=dtype, device=device)
-            self.table = torch.full((max_slots, max_pages_per_seq), -1, dtype=torch.int32, device=device)
+            self.table = torch.full((rows, max_pages_per_seq), -1, dtype=torch.int32, device=device)
+
+    def pools(self) -> dict[str, torch.Tensor]:
+        """The pools of the group's pages, [pages, numbers of a page] each, by what they hold."""
+        p = self.pages8
+        if p is not None:
+            held = (p.k.view(torch.uint8), p.v.view(torch.uint8), p.k_scale, p.v_scale, p.weight)
+            return {n: t.view(t.shape[0], -1) for n, t in zip(POOLS, held) if t is not None}
+        out = {"keys": self.k_pages.view(-1, self.page_stride)}
+        if self.v_pages is not None:
+            out["values"] = self.v_pages.view(-1, self.v_page_stride)
+        return out
+
+    def position_bytes(self) -> tuple[float, float]:
+        """What a position costs in all the group's layers: keys (with the weight it has received, where that is kept), values.
+        A scale is shared by 16 positions, so the numbers need not be whole."""
+        rows = len(self.entries) * self.key.num_kv_heads
+        if self.pages8 is not None:
+            return rows * (self.key.head_dim + 4 / 16 + (4 if self.pages8.weight is not None else 0)), rows * (self.key.value_dim + 4 / 16)
+        return rows * self.key.head_dim * self.k_pages.element_size(), rows * self.key.value_dim * self.k_pages.element_size()
 
     def offset_of(self, entry: int) -> int:
         return self.entries.index(entry) * self.layer_elems
@@ -183,6 +222,7 @@ class Slot:
     length: int = 0
     live: bool = False
     reserved: int = 0                 # positions reserved beyond length by the running step
+    dropped: int = 0                  # positions that were let go: the next token's position is length + dropped
 
 
 class PagedCache:
@@ -193,12 +233,22 @@ class PagedCache:
     """
 
     def __init__(self, needs, max_tokens: int, dtype: torch.dtype, device, page_size: int = 64,
-                 max_slots: int | None = None, max_positions: int | None = None, window_step: int = 2048):
-        """``window_step``: the most positions that one step adds to a sequence where a group keeps a window; such a
+                 max_slots: int | None = None, max_positions: int | None = None, window_step: int = 2048,
+                 kv_cache: str = "same", track_weights: bool = False):
+        """``kv_cache``: "same" (pages in the activations' type) or "e4m3" (pages of 8 bits where the mixers can read them).
+        ``track_weights``: those pages also keep the attention weight that each position receives.
+        ``window_step``: the most positions that one step adds to a sequence where a group keeps a window; such a
         group's pool is sized for ``max_slots`` windows of that reach, and whoever runs longer steps cuts them
         (``step_limit`` says so: None where no pool is smaller for it)."""
         if page_size < 1 or max_tokens < 1 or window_step < 1:
             raise CacheError("page_size, max_tokens and window_step must be positive")
+        if kv_cache not in ("same", "e4m3"):
+            raise CacheError(f"kv_cache is 'same' or 'e4m3', got {kv_cache!r}")
+        if kv_cache == "e4m3" and page_size % 64:
+            raise CacheError(f"pages of 8 bits hold a multiple of 64 positions, not {page_size}")
+        if track_weights and kv_cache != "e4m3":
+            raise CacheError("pages of 8 bits alone keep the weights that positions receive")
+        self.kv_cache, self.track_weights = kv_cache, track_weights
         self.page_size = page_size
         self.n_pages = -(-max_tokens // page_size)
         self.max_slots = min(self.n_pages, 4096) if max_slots is None else max_slots
@@ -211,11 +261,18 @@ class PagedCache:
         by_key: dict[GroupKey, list[int]] = {}
         self._entry_group: dict[int, tuple[CacheGroup, int, bool]] = {}
         self._needs = list(needs)
+        # an entry's pages are of 8 bits if its own mixer and every one that reads its cache can work on such
+        e4m3 = {e: kv_cache == "e4m3" and n.reads_e4m3 for e, (n, _s, of) in enumerate(self._needs) if n is not None and of is None}
+        for n, _state, of in self._needs:
+            if n is not None and of in e4m3:
+                e4m3[of] = e4m3[of] and n.reads_e4m3
+        if kv_cache == "e4m3" and not any(e4m3.values()):
+            raise CacheError("none of the model's layers can read pages of 8 bits")
         for e, (cache_need, _state, cache_of) in enumerate(self._needs):
             if cache_need is not None and cache_of is None:
                 by_key.setdefault(GroupKey(cache_need.num_kv_heads, cache_need.head_dim, cache_need.value_width,
                                            cache_need.window, cache_need.chunk,
-                                           cache_need.keep_first if cache_need.window is not None else 0), []).append(e)
+                                           cache_need.keep_first if cache_need.window is not None else 0, e4m3[e]), []).append(e)
         # A sequence holds, of a group with a window, the pages that its last `window` positions touch, and during a
         # step those of the step's new positions too, until the step is committed: window + window_step positions
         # lie in at most that many pages plus two.
@@ -227,7 +284,7 @@ class PagedCache:
                 for_windows = self.max_slots * (-(-(key.window + window_step) // page_size) + 2 + -(-key.keep_first // page_size))
                 if for_windows < pages:
                     pages, self.step_limit = for_windows, window_step
-            self.groups.append(CacheGroup(key, entries, pages, page_size, self.max_slots, per_seq, dtype, device))
+            self.groups.append(CacheGroup(key, entries, pages, page_size, self.max_slots, per_seq, dtype, device, track_weights))
         self._v_offset: dict[int, int] = {}
         for g in self.groups:
             for e in g.entries:
@@ -267,7 +324,7 @@ class PagedCache:
             raise CacheFull(f"all {self.max_slots} slots hold live sequences")
         i = self._free_slots.pop()
         s = self.slots[i]
-        s.length, s.live, s.reserved = 0, True, 0
+        s.length, s.live, s.reserved, s.dropped = 0, True, 0, 0
         for st in self.states.values():
             st[i].zero_()
         return i
@@ -282,7 +339,7 @@ class PagedCache:
                 g.pool.give_back(held.tolist())
                 row[:] = -1
                 g.dirty.add(slot)
-        s.live, s.length, s.reserved = False, 0, 0
+        s.live, s.length, s.reserved, s.dropped = False, 0, 0, 0
         self._free_slots.append(slot)
 
     def length(self, slot: int) -> int:
@@ -392,6 +449,8 @@ class PagedCache:
             raise CacheError(f"slot {slot} holds {s.length} positions, not {length}")
         if length == s.length:
             return
+        if s.dropped:
+            raise CacheError(f"slot {slot} has let positions go: what is left are not the first ones of what it has seen")
         if any(state is not None for _c, state, _o in self._needs):
             raise CacheError("a model with fixed-size state per sequence cannot go back to an earlier position")
         for g in self.groups:
@@ -408,13 +467,61 @@ class PagedCache:
                 g.dirty.add(slot)
         s.length = length
 
+    # ------------------------------------------------------------ positions that are let go
+    def no_eviction(self) -> str | None:
+        """Why positions cannot be let go, or None."""
+        if not self.groups or not all(g.key.e4m3 for g in self.groups):
+            return "every layer that keeps a cache has to keep one of 8 bits"
+        if not self.track_weights:
+            return "the cache does not keep the weights that positions receive (track_weights)"
+        if any(g.key.window is not None or g.key.chunk is not None for g in self.groups):
+            return "layers with a window or chunks count on the places of all positions"
+        return None
+
+    def positions_of(self, slots, places) -> list[int]:
+        """The positions of tokens at these places of the slots' sequences."""
+        return [p + self.slots[s].dropped for s, p in zip(slots, places)]
+
+    def begin_evict(self, slot: int, keep: int) -> None:
+        """Pages for ``keep`` positions of a sequence that holds more, in the spare row of every group's table."""
+        s, why = self._live(slot), self.no_eviction()
+        if why is not None:
+            raise CacheError(f"positions cannot be let go: {why}")
+        if s.reserved:
+            raise CacheError(f"slot {slot} has positions reserved for a running step")
+        if not 1 <= keep < s.length:
+            raise CacheError(f"slot {slot} holds {s.length} positions: fewer than these and at least one can stay, not {keep}")
+        n = -(-keep // self.page_size)
+        short = [g for g in self.groups if g.pool.n_free < n]
+        if short:
+            raise CacheFull(f"letting positions go needs {n} pages to copy the others to, {short[0].pool.n_free} of {short[0].pool.n_pages} are free")
+        for g in self.groups:
+            g.host_table[g.spare, :n] = g.pool.take(n)
+            g.dirty.add(g.spare)
+
+    def end_evict(self, slot: int, keep: int, done: bool = True) -> None:
+        """The spare row's pages become the sequence's (or, not ``done``, go back), and the others go back."""
+        s = self._live(slot)
+        for g in self.groups:
+            row, spare = g.host_table[slot], g.host_table[g.spare]
+            gone = row if done else spare
+            g.pool.give_back(gone[gone >= 0].tolist())
+            if done:
+                row[:] = spare
+                g.dirty.add(slot)
+            spare[:] = -1
+            g.dirty.add(g.spare)
+        if done:
+            s.dropped += s.length - keep
+            s.length = keep
+
     def export_slot(self, slot: int) -> dict:
         """What the cache holds of one sequence, on the host: its length, per group the logical pages it holds
         (first page, keys [pages, page elements], values) and per entry its row of fixed-size state."""
         s = self._live(slot)
         if s.reserved:
             raise CacheError(f"slot {slot} has positions reserved for a running step")
-        out = {"length": s.length, "page_size": self.page_size, "groups": [], "states": {}}
+        out = {"length": s.length, "page_size": self.page_size, "dropped": s.dropped, "groups": [], "states": {}}
         for g in self.groups:
             first = g.first_needed_page(s.length)
             row = g.host_table[slot]
@@ -423,9 +530,10 @@ class PagedCache:
                 raise CacheError(f"slot {slot} does not hold all pages of its {s.length} positions")
             idx = torch.tensor(pages, dtype=torch.int64, device=self.device)
             entry = {"first_page": first, "entries": list(g.entries), "key": (g.key.num_kv_heads, g.key.head_dim, g.key.value_dim, g.key.window, g.key.chunk, g.key.keep_first),
-                     "keys": g.k_pages.view(-1, g.page_stride)[idx].cpu(), "values": None}
-            if g.v_pages is not None:
-                entry["values"] = g.v_pages.view(-1, g.v_page_stride)[idx].cpu()
+                     "keys": None, "values": None}
+            if g.key.e4m3:
+                entry["key"] += (True,)
+            entry.update({name: pool[idx].cpu() for name, pool in g.pools().items()})
             out["groups"].append(entry)
         for e, st in self.states.items():
             out["states"][e] = st[slot].cpu()
@@ -439,10 +547,16 @@ class PagedCache:
             saved = tuple(d["key"])
             saved += (None,) * (5 - len(saved))
             saved += (0,) * (6 - len(saved))
-            if saved != (g.key.num_kv_heads, g.key.head_dim, g.key.value_dim, g.key.window, g.key.chunk, g.key.keep_first) or \
-                    list(d["entries"]) != list(g.entries) or d["keys"].dtype != self.dtype or \
-                    d["keys"].shape[1] != g.page_stride or (d["values"] is None) != (g.v_pages is None):
+            saved += (False,) * (7 - len(saved))
+            pools = g.pools()
+            # (weights alone may be missing or left over: a cache that does not keep them has no use for them, one that does starts them at 0)
+            if saved != (g.key.num_kv_heads, g.key.head_dim, g.key.value_dim, g.key.window, g.key.chunk, g.key.keep_first, g.key.e4m3) or \
+                    list(d["entries"]) != list(g.entries) or \
+                    any(d.get(n) is None or d[n].dtype != t.dtype or d[n].shape[1] != t.shape[1] for n, t in pools.items() if n != "weights" or d.get(n) is not None) or \
+                    (d["values"] is None) != ("values" not in pools):
                 raise CacheError("the saved sequence comes from a cache of another layout")
+        if int(data.get("dropped", 0)) and self.no_eviction() is not None:
+            raise CacheError("the saved sequence has let positions go, which this cache cannot do")
         slot = self.open()
         try:
             length = int(data["length"])
@@ -457,9 +571,9 @@ class PagedCache:
                 row = g.host_table[slot]
                 idx = torch.tensor([int(row[p]) for p in needed], dtype=torch.int64, device=self.device)
                 if idx.numel():
-                    g.k_pages.view(-1, g.page_stride)[idx] = d["keys"].to(self.device)
-                    if g.v_pages is not None:
-                        g.v_pages.view(-1, g.v_page_stride)[idx] = d["values"].to(self.device)
+                    for name, pool in g.pools().items():
+                        pool[idx] = d[name].to(self.device) if d.get(name) is not None else torch.zeros((), dtype=pool.dtype, device=self.device)
+            self.slots[slot].dropped = int(data.get("dropped", 0))
             for e, st in data["states"].items():
                 self.states[int(e)][slot].copy_(st.to(self.device))
         except BaseException:
@@ -478,7 +592,8 @@ class PagedCache:
             raise CacheError(f"schedule entry {entry} keeps no keys and values")
         g, off, owns = self._entry_group[entry]
         return KVView(g.k_pages, g.v_pages, g.table, off, g.page_size, g.page_stride, self._needs[entry][0].window, owns,
-                      self._v_offset[entry], g.v_page_stride, g.key.value_dim)
+                      self._v_offset[entry], g.v_page_stride, g.key.value_dim, g.pages8,
+                      g.entries.index(entry if owns else self._needs[entry][2]))
 
     def state(self, entry: int) -> torch.Tensor:
         if entry not in self.states:
@@ -492,7 +607,6 @@ class PagedCache:
     def bytes(self) -> int:
         n = 0
         for g in self.groups:
-            for pages in (g.k_pages, g.v_pages):
-                if pages is not None:
-                    n += pages.numel() * pages.element_size()
+            if g.table is not None:
+                n += sum(t.numel() * t.element_size() for t in g.pools().values())
         return n

@@ -8,7 +8,8 @@ DIR`` is the random-weights mode: it writes a model folder for a configuration a
 is the reference's teacher-forced perplexity (/root/reference/tools/quant.c:430-720) over a file of token ids, with its
 report and, with ``--json``, its JSON; ``--save-logits FILE`` and ``--kl-baseline FILE`` go with it as in the reference
 (:542-556, :594-636): the first writes every scored position's probabilities, the second reports the mean KL divergence
-of such a file against this run (the 32-bit path against the bfloat16 path, for instance).  ``--save-kv FILE`` and
+of such a file against this run (the 32-bit path against the bfloat16 path, for instance, or a cache in 8 bits,
+``--kv-cache e4m3``, against one that is not).  ``--save-kv FILE`` and
 ``--load-kv FILE`` are the reference's too (/root/reference/src/engine/tq_generate.c:268-362): the cache of one prompt
 saved once it has run, and a later run that starts from it with its prompt behind the saved tokens.
 """
@@ -54,6 +55,10 @@ def build_parser() -> argparse.ArgumentParser:
     ap.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"])
     ap.add_argument("--f32-weights", default="bfloat16", choices=["bfloat16", "keep"],
                     help="with --dtype bfloat16: round matrices stored in 32 bits to bfloat16 at load (default), or keep them")
+    ap.add_argument("--kv-cache", default="same", choices=["same", "e4m3"],
+                    help="keys and values are cached in --dtype (same, the default) or in 8 bits with a scale per 16 positions (e4m3)")
+    ap.add_argument("--when-full", default="end", choices=["end", "evict"],
+                    help="a sequence that reaches the context ends (default), or lets half of its positions go (needs --kv-cache e4m3)")
     ap.add_argument("--rep-penalty", type=float, default=1.1, help="repetition penalty over the last 32 tokens (default: 1.1)")
     ap.add_argument("--stop-id", type=int, action="append", default=None, help="stop token id (default: eos_token_id of config.json)")
     ap.add_argument("--random-prompt", default=None, metavar="LEN[,LEN...]", help="prompts of random token ids of these lengths")
@@ -106,7 +111,9 @@ def main(argv=None) -> int:
     t0 = time.time()
     model = Model(args.model, temperature=args.temperature, top_p=args.top_p, max_tokens=args.max_tokens,
                   context_length=args.ctx, dtype=args.dtype, seed=args.seed, rep_penalty=args.rep_penalty,
-                  max_batch=args.max_batch, stop_tokens=args.stop_id, f32_matrices=args.f32_weights)
+                  max_batch=args.max_batch, stop_tokens=args.stop_id, f32_matrices=args.f32_weights,
+                  kv_cache=args.kv_cache, when_full=args.when_full)
+    kv_type = args.dtype if args.kv_cache == "same" else args.kv_cache
     print(f"loaded {args.model} in {time.time() - t0:.1f}s ({args.dtype}, context {model.context_length})", file=sys.stderr)
     if args.bench_memory or args.bench_prefill:
         # the reference's two small benchmarks (/root/reference/tools/quant.c:726-800, :804-860): one token, its token
@@ -115,7 +122,7 @@ def main(argv=None) -> int:
         tok = min(1, eng.vocab_size - 1)
         if args.bench_memory:
             print("\n=== Memory Bandwidth Benchmark ===", file=sys.stderr)
-            print(f"KV type: {args.dtype}", file=sys.stderr)
+            print(f"KV type: {kv_type}", file=sys.stderr)
             print(f"{'Context':<12} {'Tok/s':<12} {'Time(s)':<12}", file=sys.stderr)
             print("-------- -------- --------", file=sys.stderr)
             for ctx in (10, 50, 100, 200, 500):
@@ -149,7 +156,7 @@ def main(argv=None) -> int:
                 torch.cuda.synchronize()
                 elapsed = time.time() - t1
                 eng.close(slot)
-            name = f"{args.dtype} (no quant)"
+            name = f"{args.dtype} (no quant)" if args.kv_cache == "same" else kv_type
             print(f"{name:<28} {n / elapsed:<12.1f} {elapsed:<12.3f}", file=sys.stderr)
             print(f"PREFILL_CSV:{name},{n},{n / elapsed:.2f},{elapsed:.4f}", file=sys.stderr)
             print("===============================", file=sys.stderr)
@@ -167,7 +174,7 @@ def main(argv=None) -> int:
         print("\n=== Perplexity Results ===", file=sys.stderr)
         print(f"File:         {args.ppl}", file=sys.stderr)
         print(f"Tokens:       {res['tokens']} (evaluated {res['tokens_evaluated']})", file=sys.stderr)
-        print(f"KV type:      {args.dtype}", file=sys.stderr)
+        print(f"KV type:      {kv_type}", file=sys.stderr)
         print(f"Avg NLL:      {res['avg_nll']:.6f}", file=sys.stderr)
         print(f"Perplexity:   {res['perplexity']:.4f}", file=sys.stderr)
         print(f"Time:         {elapsed:.1f}s ({rate:.1f} tok/s)", file=sys.stderr)
@@ -179,7 +186,7 @@ def main(argv=None) -> int:
         print(f"PPL_CSV:{res['tokens_evaluated']},{res['avg_nll']:.6f},{res['perplexity']:.4f}", file=sys.stderr)
         if args.json:
             print(json.dumps({"model": args.model, "benchmark": args.ppl, "tokens": res["tokens"],
-                              "tokens_evaluated": res["tokens_evaluated"], "kv_type": args.dtype,
+                              "tokens_evaluated": res["tokens_evaluated"], "kv_type": kv_type,
                               "perplexity": round(res["perplexity"], 4), "avg_nll": round(res["avg_nll"], 6),
                               "elapsed_s": round(elapsed, 2), "tok_per_s": round(rate, 1),
                               **({"mean_kl": res["mean_kl"], "kl_tokens": res["kl_tokens"]} if args.kl_baseline else {})},
@@ -228,35 +235,34 @@ def main(argv=None) -> int:
             print(f"[{i}] {' '.join(str(t) for t in r.tokens)}  ({r.finish_reason})")
     if n_generated > 0 and elapsed > 0:
         print(f"{n_generated} tokens in {elapsed:.1f}s ({n_generated / elapsed:.1f} tok/s, {len(prompts)} sequences, "
-              f"weights={args.dtype}, kv={args.dtype})", file=sys.stderr)
+              f"weights={args.dtype}, kv={kv_type})", file=sys.stderr)
     if args.memory and n_generated > 0:
-        # the reference's report (/root/reference/tools/quant.c:1382-1461), for a cache that is not compressed: what a
+        # the reference's report (/root/reference/tools/quant.c:1382-1461), what a
         # token costs in every layer that keeps keys and values, against keys and values in 16-bit floats
         cache = model.engine.cache
-        esz = 4 if args.dtype == "float32" else 2
         # what the cache held of each sequence when it ended: a token that ended a sequence was never run, and a group
         # with a window has given its older pages back
         n_tok = sum(r.cached_positions for r in results) or sum(len(p) + len(r.tokens) for p, r in zip(prompts, results))
-        k_per = sum(len(g.entries) * g.key.num_kv_heads * g.key.head_dim * esz for g in cache.groups)
-        v_per = sum(len(g.entries) * g.key.num_kv_heads * g.key.value_dim * esz for g in cache.groups)
-        f16_per = (k_per + v_per) // esz * 2
+        k_per = sum(g.position_bytes()[0] for g in cache.groups)
+        v_per = sum(g.position_bytes()[1] for g in cache.groups)
+        in16 = [len(g.entries) * g.key.num_kv_heads * (g.key.head_dim + g.key.value_dim) * 2 for g in cache.groups]
+        f16_per = sum(in16)
         if all(r.pages_held for r in results):
             held = [sum(min(r.cached_positions, r.pages_held[i] * cache.page_size) for r in results)
                     for i in range(len(cache.groups))]
-            total = sum(len(g.entries) * g.key.num_kv_heads * (g.key.head_dim + g.key.value_dim) * esz * n
-                        for g, n in zip(cache.groups, held))
-            total16 = total // esz * 2
+            total = int(sum(sum(g.position_bytes()) * n for g, n in zip(cache.groups, held)))
+            total16 = sum(per * n for per, n in zip(in16, held))
         else:
-            total, total16 = (k_per + v_per) * n_tok, f16_per * n_tok
+            total, total16 = int((k_per + v_per) * n_tok), f16_per * n_tok
         ratio = total16 / total if total else 0.0
         print("\n=== KV Cache Memory Stats ===", file=sys.stderr)
         print(f"Tokens in cache:      {n_tok}", file=sys.stderr)
         print("Model config:         " + "; ".join(
             f"{len(g.entries)} layers, {g.key.num_kv_heads} kv_heads, head_dim={g.key.head_dim}"
             + (f", window={g.key.window}" if g.key.window else "") for g in cache.groups), file=sys.stderr)
-        print(f"KV type:              {args.dtype}", file=sys.stderr)
-        print(f"Per-token K ({args.dtype}): {k_per / 1024:.2f} KB", file=sys.stderr)
-        print(f"Per-token V ({args.dtype}): {v_per / 1024:.2f} KB", file=sys.stderr)
+        print(f"KV type:              {kv_type}", file=sys.stderr)
+        print(f"Per-token K ({kv_type}): {k_per / 1024:.2f} KB", file=sys.stderr)
+        print(f"Per-token V ({kv_type}): {v_per / 1024:.2f} KB", file=sys.stderr)
         print(f"Per-token K+V total:  {(k_per + v_per) / 1024:.2f} KB", file=sys.stderr)
         print(f"Per-token K+V (FP16): {f16_per / 1024:.2f} KB", file=sys.stderr)
         print(f"Total K+V:            {total / 1024 / 1024:.2f} MB", file=sys.stderr)
@@ -273,7 +279,7 @@ def main(argv=None) -> int:
         from .csrc import ops
         from .engine.step import Engine
         eng = Engine(model._model, max_tokens=sum(-(-(len(p) + 17) // 64) * 64 for p in prompts), page_size=64,
-                     max_slots=len(prompts), use_graphs=False)
+                     max_slots=len(prompts), use_graphs=False, kv_cache=args.kv_cache, track_weights=args.when_full == "evict")
         eng.side_stream = None
         slots = eng.open(len(prompts))
         print("[Profile] steps are timed eagerly on one stream, an event behind every launch; generation replays its "

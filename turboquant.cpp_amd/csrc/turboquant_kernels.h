@@ -304,6 +304,22 @@ int tq_attn_prep_kv_write(float* qkv, int64_t ld, const int* positions, const in
         const void* lambda, void* q_out, void* k_pool, void* v_pool, int page_size, int64_t page_stride, int T, int nh,
         int nkv, int hd, int write_kv, const int* cu_seqlens, const int* slots, const int* start, int B, int max_new,
         hipStream_t st);
+// cache_e4m3.hip, attention_e4m3.hip: pages in 8 bits (cache_e4m3.h), what writes and reads them, and which positions stay
+int tq_e4m3_write(const float* x, int64_t ld, const void* bias, int bias_type, const int* positions, const float* inv_freq,
+        int pairing, int rot, float amp, const int* cu, const int* slots, const int* start, void* q, int T, int B,
+        int max_new, int nh, int nkv, int hd, void* k, void* v, float* k_scale, float* v_scale, float* weight,
+        const int* table, int bt_stride, int page_size, int heads, int head0, hipStream_t st);
+int64_t tq_e4m3_attention_scratch(int T, int B, int nh, int nkv, int hd, int max_new, int max_end, int decode, int weights);
+int tq_e4m3_attention(const void* q, void* out, const int* cu, const int* slots, const int* start, int T, int B, int nh, int nkv,
+        int hd, int window, float scale, float softcap, const float* r1, const float* r2, int chunk,
+        const float* sink, const void* k, const void* v, const float* k_scale, const float* v_scale, float* weight,
+        const int* table, int bt_stride, int page_size, int heads, int head0, float* scratch, int decode, int max_new,
+        int max_end, hipStream_t st);
+int tq_e4m3_choose(const int* slots, const int* lengths, int B, int max_length, int keep, int first, int recent, int* kept,
+        const float* weight, const int* table, int slots_of_table, int bt_stride, int page_size, int heads, hipStream_t st);
+int tq_e4m3_move(const int* src, const int* dst, int B, const int* kept, int keep, int hd, void* k, void* v, float* k_scale,
+        float* v_scale, float* weight, const int* table, int slots_of_table, int bt_stride, int page_size, int heads,
+        hipStream_t st);
 // sampling.hip: greedy choice, negative log-likelihood, repetition penalty, temperature and top-p (both libraries; the two *_static entry points are declared in no_alloc.h)
 int tq_argmax(const float* logits, int R, int V, int* out, hipStream_t st);
 int tq_nll(const float* logits, int R, int V, const int* target, float* out, hipStream_t st);

@@ -17,7 +17,7 @@ import torch
 class StepBatch:
     slots: list[int]                  # slot of each sequence of the step
     n_new: list[int]                  # tokens each sequence brings
-    start: list[int]                  # position of each sequence's first new token
+    start: list[int]                  # place in the cache of each sequence's first new token (its position, if none were let go)
     n_tokens: int
     tokens: torch.Tensor              # int32 [T]
     positions: torch.Tensor           # int32 [T]
@@ -75,10 +75,11 @@ class StepBatch:
                 "max_new": self.max_new, "min_new": min(self.n_new), "max_end": self.max_end, "decode": self.is_decode}
 
 
-def pack_step(slots, starts, token_lists, wants, device) -> StepBatch:
+def pack_step(slots, starts, token_lists, wants, device, ahead=None) -> StepBatch:
     """Packs per-sequence token lists into the arrays of a step and sends them to the device in one copy.
 
-    ``wants[i]`` lists the places among sequence i's new tokens whose logits are asked for."""
+    ``wants[i]`` lists the places among sequence i's new tokens whose logits are asked for; ``ahead[i]`` is how far its tokens'
+    positions are ahead of their places in the cache (positions that were let go; None: not at all)."""
     n_new = [len(t) for t in token_lists]
     B, T = len(slots), sum(n_new)
     R = sum(len(w) for w in wants)
@@ -95,7 +96,8 @@ def pack_step(slots, starts, token_lists, wants, device) -> StepBatch:
     for i, (slot, start, toks, want) in enumerate(zip(slots, starts, token_lists, wants)):
         n = len(toks)
         views["tokens"][off:off + n] = toks
-        views["positions"][off:off + n] = np.arange(start, start + n, dtype=np.int32)
+        first = start if ahead is None else start + ahead[i]
+        views["positions"][off:off + n] = np.arange(first, first + n, dtype=np.int32)
         views["slot_of_token"][off:off + n] = slot
         views["cu_seqlens"][i] = off
         for w in want:

@@ -9,11 +9,14 @@ and pages back at once and the others go on; when more requests wait than a batc
 batch.  Where the reference shifts a full context (:456-514), a sequence here ends with reason ``"context"``:
 when it reaches the positions a sequence may hold, and also when the cache's pages run out while several
 sequences grow (the longest of those that need a page ends, its pages let the others go on); a prompt that
-finds no room beside the others of its batch waits for the next batch.  The decisions are kept apart from
+finds no room beside the others of its batch waits for the next batch.  With ``when_full="evict"`` a sequence that
+reaches the positions it may hold lets half of them go instead (``Engine.evict``: those that have received little attention) and
+goes on.  The decisions are kept apart from
 the device work (``SequenceTrack``) so that they are tested without one.
 """
 from __future__ import annotations
 
+import sys
 from collections import deque
 from dataclasses import dataclass, field
 from typing import Callable, Sequence
@@ -36,6 +39,8 @@ class GenerationOptions:
     loop_detection: bool = True               # stop when a 4-gram has repeated three times
     max_batch: int = 8
     on_token: Callable[[int, int], None] | None = None   # (request index, token)
+    # a sequence that holds all the positions it may: "end" (with reason "context") or "evict" (half of them are let go)
+    when_full: str = "end"
 
     def sampling(self) -> SamplingOptions:
         return SamplingOptions(self.temperature, self.top_p, self.seed, self.rep_penalty, self.rep_window)
@@ -45,7 +50,8 @@ class GenerationOptions:
 class GenerationResult:
     tokens: list[int]
     finish_reason: str            # "stop" (end token), "length" (max_tokens), "context" (cache or model limit), "loop"
-    cached_positions: int = 0     # positions the cache held for the sequence when it ended (a token that ended it was not run)
+    # positions the cache held for the sequence when it ended (a token that ended it was not run; without those let go)
+    cached_positions: int = 0
     pages_held: tuple = ()        # pages it held then, per cache group (a group with a window has given the older ones back)
 
 
@@ -126,6 +132,14 @@ class SequenceTrack:
         return True
 
 
+def kept_when_full(max_positions: int) -> tuple[int, int, int]:
+    """How many of its ``max_positions`` a full sequence keeps: half, among them the first four and, of what is left of that
+    half, the last half."""
+    keep = max(1, max_positions // 2)
+    first = min(4, keep - 1)
+    return keep, first, (keep - first + 1) // 2
+
+
 def plan_batches(n_requests: int, max_batch: int) -> list[list[int]]:
     """Requests in order, ``max_batch`` at a time."""
     if max_batch < 1:
@@ -142,6 +156,10 @@ def generate(engine, prompts: Sequence[Sequence[int]], options: GenerationOption
         raise ValueError("max_batch must be at least 1")
     if o.max_tokens < 1:
         return [GenerationResult([], "length") for _ in prompts]
+    if o.when_full not in ("end", "evict"):
+        raise ValueError(f"when_full is 'end' or 'evict', got {o.when_full!r}")
+    if o.when_full == "evict" and engine.no_eviction() is not None:
+        raise ValueError(f"when_full='evict': {engine.no_eviction()}")
     sampler = Sampler(o.sampling(), engine.model.act, engine.device)
     results: list[GenerationResult | None] = [None] * len(prompts)
     max_pos = engine.cache.max_positions
@@ -154,6 +172,11 @@ def generate(engine, prompts: Sequence[Sequence[int]], options: GenerationOption
         held = tuple(int((g.host_table[slot] >= 0).sum()) for g in engine.cache.groups)
         results[r] = GenerationResult(tracks[r].out, tracks[r].finish_reason, engine.length(slot), held)
         engine.close([slot])
+
+    def make_room(slots):
+        """Before a step of one token: those that hold all they may let half go."""
+        if o.when_full == "evict":
+            engine.evict([s for s in slots if engine.length(s) >= max_pos], *kept_when_full(max_pos))
 
     while waiting:
         batch = []
@@ -169,7 +192,8 @@ def generate(engine, prompts: Sequence[Sequence[int]], options: GenerationOption
         if not batch:
             continue
         slots = engine.open(len(batch))
-        tracks = {r: SequenceTrack.start(r, prompts[r], o, max_pos) for r in batch}
+        most = max_pos if o.when_full == "end" else sys.maxsize      # what a track counts: positions seen, let go or not
+        tracks = {r: SequenceTrack.start(r, prompts[r], o, most) for r in batch}
         samp = {r: sampler.new_sequence(r, list(prompts[r])) for r in batch}
         slot_of = dict(zip(batch, slots))
         live = list(batch)
@@ -201,6 +225,7 @@ def generate(engine, prompts: Sequence[Sequence[int]], options: GenerationOption
                 if ahead:
                     feed = ids if len(ahead) == len(live) else ids[torch.tensor(ahead, dtype=torch.int64, device=ids.device)]
                     try:
+                        make_room([slot_of[live[i]] for i in ahead])
                         next_logits = engine.step_from_device([slot_of[live[i]] for i in ahead], feed)
                     except CacheFull:
                         # no page to run ahead with: a sequence that ends on this token may give one back, so the
@@ -217,6 +242,7 @@ def generate(engine, prompts: Sequence[Sequence[int]], options: GenerationOption
                 if going and not ahead:
                     while going:
                         try:
+                            make_room([slot_of[live[i]] for i in going])
                             logits = engine.step([slot_of[live[i]] for i in going], [[tokens[i]] for i in going])
                             break
                         except CacheFull:
@@ -240,7 +266,7 @@ def continue_in_slot(engine, slot: int, history: Sequence[int], options: Generat
     """One sequence that outlives the call, as the reference's chat keeps its state between turns
     (/root/reference/quant.h:17634-17700): ``history`` is everything the sequence has seen and is to see, the slot's
     cache holds its first ``engine.length(slot)`` tokens (fewer than all of them), the rest is run as one prompt step
-    and a continuation is generated.  The slot stays open; afterwards its cache holds the history and the generated
+    and a continuation is generated.  Nothing is let go: the history is what the cache holds.  The slot stays open; afterwards its cache holds the history and the generated
     tokens but the last, if that one ended the turn by its number (``engine.length(slot)`` says how many)."""
     o = options or GenerationOptions()
     cached = engine.length(slot)

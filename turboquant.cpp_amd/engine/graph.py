@@ -45,13 +45,13 @@ class DecodeGraph:
         self.pool = pool
 
     def fill(self, slots, starts, tokens) -> None:
-        """``tokens``: a list, or an int32 tensor on the device that is copied in behind the other arrays."""
+        """``starts``: places in the cache.  ``tokens``: a list, or an int32 tensor on the device that is copied in behind the other arrays."""
         self.copied.synchronize()          # the last copy out of the pinned array has been done
         h, off = self.host_np, self.offsets
         on_device = isinstance(tokens, torch.Tensor)
         if not on_device:
             h[off["tokens"][0]:off["tokens"][1]] = tokens
-        h[off["positions"][0]:off["positions"][1]] = starts
+        h[off["positions"][0]:off["positions"][1]] = self.engine.cache.positions_of(slots, starts)
         h[off["slot_of_token"][0]:off["slot_of_token"][1]] = slots
         h[off["slots"][0]:off["slots"][1]] = slots
         h[off["start"][0]:off["start"][1]] = starts

@@ -126,11 +126,14 @@ class CausalLM:
         return needs
 
     def new_cache(self, max_tokens: int, page_size: int = 64, max_slots: int | None = None,
-                  max_positions: int | None = None, window_step: int = 2048) -> PagedCache:
-        """``max_positions``: the most positions a sequence may reach, if that is to be fewer than the model allows."""
+                  max_positions: int | None = None, window_step: int = 2048, kv_cache: str = "same",
+                  track_weights: bool = False) -> PagedCache:
+        """``max_positions``: the most positions a sequence may reach, if that is to be fewer than the model allows; the other
+        arguments are ``PagedCache``'s."""
         limit = self.plan.max_positions if max_positions is None else min(max_positions, self.plan.max_positions)
         return PagedCache(self.cache_needs(), max_tokens, self.act_dtype, self.device, page_size=page_size,
-                          max_slots=max_slots, max_positions=limit, window_step=window_step)
+                          max_slots=max_slots, max_positions=limit, window_step=window_step, kv_cache=kv_cache,
+                          track_weights=track_weights)
 
     # ------------------------------------------------------------ forward
     def forward(self, ctx: StepContext) -> torch.Tensor:

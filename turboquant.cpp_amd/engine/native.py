@@ -42,6 +42,8 @@ class NativeModel:
             if block.state_need() is not None or block.cache_need() is None:
                 raise ValueError("the step executor runs layers that keep keys and values and no state of their own")
             kv = cache.kv(e)
+            if kv.pages8 is not None:
+                raise ValueError("the step executor's attention reads pages of the activations' type")
             if kv.v_pages is None or kv.v_layer_offset != kv.layer_offset or kv.v_page_stride != kv.page_stride:
                 raise ValueError("the step executor's attention keeps values as wide as its keys")
             entries.append(host_api.EntryDesc(sched.layer, kv.k_pages.data_ptr(), kv.v_pages.data_ptr(), kv.table.data_ptr(),

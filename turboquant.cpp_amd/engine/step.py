@@ -29,13 +29,17 @@ class Engine:
     each sequence rounded up to whole pages of ``page_size``."""
 
     def __init__(self, model: CausalLM, max_tokens: int, page_size: int = 64, max_slots: int | None = None,
-                 use_graphs: bool = True, max_positions: int | None = None, window_step: int = 2048):
-        """``max_positions``: the most positions one sequence may reach (default and upper bound: the model's).
+                 use_graphs: bool = True, max_positions: int | None = None, window_step: int = 2048, kv_cache: str = "same",
+                 track_weights: bool = False):
+        """``kv_cache`` "e4m3": keys and values are kept in 8 bits by the layers that can read them (at least one has to), "same":
+        in the activations' type.  ``track_weights``: those layers also keep the attention weight that every cached position
+        receives, by which ``evict`` chooses (it costs a second pass of the attention).
+        ``max_positions``: the most positions one sequence may reach (default and upper bound: the model's).
         ``window_step``: layers that keep a window have pages for their windows and for this many new positions per
         sequence; a step that brings a sequence more is run in cuts of that length."""
         self.model = model
         self.cache = model.new_cache(max_tokens, page_size=page_size, max_slots=max_slots, max_positions=max_positions,
-                                     window_step=window_step)
+                                     window_step=window_step, kv_cache=kv_cache, track_weights=track_weights)
         self.device = model.device
         self.vocab_size = model.plan.vocab_size
         # decode steps are replayed as HIP graphs where a GPU runs them
@@ -106,7 +110,7 @@ class Engine:
                         all_rows[torch.tensor(rows, dtype=torch.int64, device=self.device)] if rows else \
                         torch.empty((0, self.vocab_size), dtype=torch.float32, device=self.device)
             if logits is None:
-                logits = self._eager(pack_step(slots, starts, token_lists, wants, self.device))
+                logits = self._eager(self._pack(slots, starts, token_lists, wants))
         except BaseException:
             self._unreserve(slots)
             raise
@@ -156,7 +160,7 @@ class Engine:
         try:
             logits = self.graphs.run(slots, starts, tokens) if self.graphs is not None and self.layer_hook is None else None
             if logits is None:
-                batch = pack_step(slots, starts, [[0]] * len(slots), [[0]] * len(slots), self.device)
+                batch = self._pack(slots, starts, [[0]] * len(slots), [[0]] * len(slots))
                 batch.tokens.copy_(tokens)
                 logits = self._eager(batch)
         except BaseException:
@@ -165,6 +169,49 @@ class Engine:
         for slot in slots:
             self.cache.commit(slot)
         return logits
+
+    def _pack(self, slots, starts, token_lists, wants):
+        ahead = [p - s for p, s in zip(self.cache.positions_of(slots, starts), starts)]
+        return pack_step(slots, starts, token_lists, wants, self.device, ahead if any(ahead) else None)
+
+    # ------------------------------------------------------------ positions that are let go
+    def no_eviction(self) -> str | None:
+        """Why ``evict`` is not possible with this model and cache, or None."""
+        if self.model.position_table is not None:
+            return "the model has a learned vector for each of a limited number of positions"
+        if any(getattr(p, "has_distance_bias", False) for p in self.model.parts()):
+            return "a layer's scores depend on how far apart two places are"
+        return self.cache.no_eviction()
+
+    def evict(self, slots: list[int], keep: int, first: int = 4, recent: int | None = None) -> None:
+        """Lets positions of every sequence in ``slots`` go that holds more than ``keep``: every layer and kv head keeps the first
+        ``first`` of them, the last ``recent`` (default: half of ``keep``), and of the others those that have received the most
+        attention since they were written, ``keep`` in all.  Keys stay rotated as they were, and later tokens go on at the positions
+        that they would have had.  Needs pages for ``keep`` positions until each sequence is done (``CacheFull`` otherwise)."""
+        why = self.no_eviction()
+        if why is not None:
+            raise StepError(f"positions cannot be let go: {why}")
+        if len(set(slots)) != len(slots):
+            raise StepError("a slot appears twice among those to let positions go")
+        recent = keep // 2 if recent is None else recent
+        if keep < 1 or first < 0 or recent < 0 or first + recent > keep:
+            raise StepError(f"the first {first} and last {recent} positions must lie within the {keep} that stay")
+        for slot in slots:
+            length = self.length(slot)
+            if length <= keep:
+                continue
+            self.cache.begin_evict(slot, keep)
+            done = False
+            try:
+                self.cache.sync()
+                for g in self.cache.groups:
+                    src, dst, n = torch.tensor([[slot], [g.spare], [length]], dtype=torch.int32).to(self.device)
+                    kept = ops.evict_choose(g.pages8, src, n, length, keep, first=first, recent=recent, act=self.model.act)
+                    ops.evict_move(g.pages8, src, dst, kept, act=self.model.act)
+                done = True
+            finally:
+                self.cache.end_evict(slot, keep, done)
+                self.cache.sync()
 
     def _reserve(self, slots, counts) -> list[int]:
         """Room for ``counts[i]`` more positions in each slot, or none at all; returns where each sequence goes on."""

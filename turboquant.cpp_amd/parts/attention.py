@@ -30,6 +30,9 @@ sigmoid(score + b_h), b a learned number per head, and the weights are not norma
 ``row_norm_eps`` (queries and keys are RMS-normed before the rotation over all their heads together, with a weight per number
 of the whole projection); ``values_are_keys`` (there is no value matrix: the values are the keys as they were projected, before
 norm and rotation); ``unit_sink`` (the softmax's denominator also holds 1: a sink whose score is 0, the same for every head).
+Where the cache keeps 8 bits (``KVView.pages8``) keys and values are written as e4m3 codes behind the same product, norm and
+rotation, and the scores are taken from the codes; a norm behind the rotation or over all heads, normed or mixed values, sigmoid
+weights and kept first positions have no such form (``CacheNeed.reads_e4m3``).
 With ``separate_qkv`` the heads are laid out at a kernel width that is the larger of key and value width rounded up to
 16: the added rows and columns of the matrices are zeros, which change no score and no output, and every head size
 then runs on the matrix-core kernels of both libraries.
@@ -228,8 +231,10 @@ class GroupedQueryAttention(Part):
         return {"position": self.position}
 
     def cache_need(self) -> CacheNeed:
+        reads_e4m3 = (self.head_dim % 16 == 0 and self.head_dim <= 256 and self.row_norm_eps is None and self.rotated_norm_eps is None
+                      and self.value_norm_eps is None and self.value_mix is None and not self.has_sigmoid_bias and not self.keep_first)
         return CacheNeed(self.num_kv_heads, self.head_dim, self.cache_window, chunk=self.chunk,
-                         keep_first=self.keep_first if self.cache_window is not None else 0)
+                         keep_first=self.keep_first if self.cache_window is not None else 0, reads_e4m3=reads_e4m3)
 
     def state_need(self):
         return None
@@ -290,7 +295,7 @@ class GroupedQueryAttention(Part):
         """A decode step's queries, keys and values for another launch to lay out (``read_out`` then takes the queries), or None
         where more than that stands between the product and the cache."""
         b, kv = ctx.batch, ctx.kv(entry)
-        if not b.is_decode or not kv.owns or self.position.rotary_dim != 0:
+        if not b.is_decode or not kv.owns or self.position.rotary_dim != 0 or kv.pages8 is not None:
             return None
         q = torch.empty((proj.shape[0], self.q_size), dtype=kv.k_pages.dtype, device=proj.device)
         return ops.KVWrite(proj, b.positions, kv.table, kv.k_pages, kv.v_pages, kv.layer_offset, kv.page_size, kv.page_stride,
@@ -300,6 +305,9 @@ class GroupedQueryAttention(Part):
         """What follows the product of the layer's input, up to the output product: rotation and cache write (done already where
         ``q`` gives the queries) and attention."""
         b, kv = ctx.batch, ctx.kv(entry)
+        if kv.pages8 is not None:
+            o = self._read_e4m3(proj, ctx, b, kv)
+            return o if out is None else out.copy_(o)
         if q is None:
             q = ops.rope_kv_write(proj, b.positions, b.slot_of_token, kv.table, self.position.table(ctx.device),
                                   self.position.pairing_code, self.position.rotary_dim, kv.k_pages if kv.owns else None,
@@ -312,6 +320,8 @@ class GroupedQueryAttention(Part):
     def forward(self, normed, ctx, entry):
         b, kv = ctx.batch, ctx.kv(entry)
         amplitude = getattr(self.position, "amplitude", 1.0)
+        if kv.pages8 is not None:
+            return self._forward_e4m3(normed, ctx, b, kv)
         if self.row_norm_eps is not None:
             return self._forward_row_norm(normed, ctx, b, kv, amplitude)
         if (self.rotated_norm_eps is not None or self.has_head_gate or self.shares_kv or amplitude != 1.0
@@ -330,6 +340,37 @@ class GroupedQueryAttention(Part):
         o = ops.attention(q, kv.k_pages, kv.v_pages, kv.layer_offset, b.positions, b.slot_of_token, kv.table,
                           kv.page_size, kv.page_stride, self.num_heads, self.num_kv_heads, self.head_dim,
                           self.window, self.scale, ctx.act, runs=b.runs(), **self._score_options())
+        return ops.gemm(o, self.out_weight, ctx.act, bias=self.out_bias, partial_sums=True)
+
+    def _read_e4m3(self, qkv, ctx, b, kv, bias=None):
+        """What follows the product where the cache keeps 8 bits: ``bias``, rotation and the write as codes, then attention, which
+        adds to the weights that positions receive if the pages keep them."""
+        if not kv.owns:      # another layer's cache is read: the queries alone are of use
+            qkv, bias = qkv[:, :self.q_size], None if bias is None else bias[:self.q_size]
+        q = ops.rope_kv_write_e4m3(qkv, b.positions, self.position.table(ctx.device), self.position.pairing_code, self.position.rotary_dim,
+                                   kv.pages8, kv.layer, self.num_heads, ctx.act, b.runs(), bias=bias,
+                                   amplitude=getattr(self.position, "amplitude", 1.0), write=kv.owns)
+        return ops.attention_e4m3(q, kv.pages8, kv.layer, self.num_heads, self.window, self.scale, ctx.act, b.runs(),
+                                  add_weights=kv.pages8.weight is not None, **self._score_options())
+
+    def _forward_e4m3(self, normed, ctx, b, kv):
+        """The form over a cache of 8 bits: the product (q | k | v | gate rows), the norm of the heads where there is one, bias,
+        rotation and cache write in one launch, attention, the gate per head, the output product."""
+        if kv.owns and self.shares_kv:
+            raise ValueError("an attention without keys and values has no cache of its own")
+        H, G, D = self.num_heads, 0 if self.shares_kv else self.num_kv_heads, self.head_dim
+        normed_heads = self.qk_norm_eps is not None
+        proj = ops.gemm(normed, self.qkv_weight, ctx.act, bias=self.qkv_bias if normed_heads else None)
+        width = (H + 2 * G) * D
+        bias = None if normed_heads or self.qkv_bias is None else self.qkv_bias[:width]
+        if normed_heads:
+            if proj.shape[1] != width:
+                raise ValueError("the norm of the heads before the rotation does not go with a gate per head")
+            ops.head_rmsnorm(proj, self.q_norm, None if self.shares_kv else self.k_norm, self.qk_norm_eps, H, G, D, ctx.act,
+                             norm_dim=self.key_dim)
+        o = self._read_e4m3(proj[:, :width], ctx, b, kv, bias)
+        if self.has_head_gate:
+            ops.gate_heads(o, proj[:, width:width + H], H, "sigmoid", ctx.act)
         return ops.gemm(o, self.out_weight, ctx.act, bias=self.out_bias, partial_sums=True)
 
     def _forward_row_norm(self, normed, ctx, b, kv, amplitude):

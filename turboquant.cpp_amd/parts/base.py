@@ -64,6 +64,7 @@ class CacheNeed:
     value_dim: int | None = None
     chunk: int | None = None
     keep_first: int = 0
+    reads_e4m3: bool = False      # the mixer can work on pages of 8 bits (ops.E4m3Pages), where the cache is asked to keep such
 
     @property
     def value_width(self) -> int:
