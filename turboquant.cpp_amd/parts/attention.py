@@ -31,8 +31,8 @@ sigmoid(score + b_h), b a learned number per head, and the weights are not norma
 of the whole projection); ``values_are_keys`` (there is no value matrix: the values are the keys as they were projected, before
 norm and rotation); ``unit_sink`` (the softmax's denominator also holds 1: a sink whose score is 0, the same for every head).
 Where the cache keeps 8 bits (``KVView.pages8``) keys and values are written as e4m3 codes behind the same product, norm and
-rotation, and the scores are taken from the codes; a norm behind the rotation or over all heads, normed or mixed values, sigmoid
-weights and kept first positions have no such form (``CacheNeed.reads_e4m3``).
+rotation, and the scores are taken from the codes; a norm behind the rotation or over all heads, a gate per head, a mixer without
+keys and values, normed or mixed values, sigmoid weights and kept first positions have no such form (``CacheNeed.reads_e4m3``).
 With ``separate_qkv`` the heads are laid out at a kernel width that is the larger of key and value width rounded up to
 16: the added rows and columns of the matrices are zeros, which change no score and no output, and every head size
 then runs on the matrix-core kernels of both libraries.
@@ -232,7 +232,8 @@ class GroupedQueryAttention(Part):
 
     def cache_need(self) -> CacheNeed:
         reads_e4m3 = (self.head_dim % 16 == 0 and self.head_dim <= 256 and self.row_norm_eps is None and self.rotated_norm_eps is None
-                      and self.value_norm_eps is None and self.value_mix is None and not self.has_sigmoid_bias and not self.keep_first)
+                      and not self.has_head_gate and not self.shares_kv and self.value_norm_eps is None and self.value_mix is None
+                      and not self.has_sigmoid_bias and not self.keep_first)
         return CacheNeed(self.num_kv_heads, self.head_dim, self.cache_window, chunk=self.chunk,
                          keep_first=self.keep_first if self.cache_window is not None else 0, reads_e4m3=reads_e4m3)
 
@@ -354,23 +355,15 @@ class GroupedQueryAttention(Part):
                                   add_weights=kv.pages8.weight is not None, **self._score_options())
 
     def _forward_e4m3(self, normed, ctx, b, kv):
-        """The form over a cache of 8 bits: the product (q | k | v | gate rows), the norm of the heads where there is one, bias,
-        rotation and cache write in one launch, attention, the gate per head, the output product."""
-        if kv.owns and self.shares_kv:
-            raise ValueError("an attention without keys and values has no cache of its own")
-        H, G, D = self.num_heads, 0 if self.shares_kv else self.num_kv_heads, self.head_dim
-        normed_heads = self.qk_norm_eps is not None
-        proj = ops.gemm(normed, self.qkv_weight, ctx.act, bias=self.qkv_bias if normed_heads else None)
-        width = (H + 2 * G) * D
-        bias = None if normed_heads or self.qkv_bias is None else self.qkv_bias[:width]
-        if normed_heads:
-            if proj.shape[1] != width:
-                raise ValueError("the norm of the heads before the rotation does not go with a gate per head")
-            ops.head_rmsnorm(proj, self.q_norm, None if self.shares_kv else self.k_norm, self.qk_norm_eps, H, G, D, ctx.act,
+        """The form over a cache of 8 bits: the product, with the norm of the heads its bias and that norm, (bias,) rotation and
+        cache write in one launch, attention, the output product."""
+        if self.qk_norm_eps is None:
+            o = self._read_e4m3(ops.gemm(normed, self.qkv_weight, ctx.act), ctx, b, kv, self.qkv_bias)
+        else:
+            qkv = ops.gemm(normed, self.qkv_weight, ctx.act, bias=self.qkv_bias)
+            ops.head_rmsnorm(qkv, self.q_norm, self.k_norm, self.qk_norm_eps, self.num_heads, self.num_kv_heads, self.head_dim, ctx.act,
                              norm_dim=self.key_dim)
-        o = self._read_e4m3(proj[:, :width], ctx, b, kv, bias)
-        if self.has_head_gate:
-            ops.gate_heads(o, proj[:, width:width + H], H, "sigmoid", ctx.act)
+            o = self._read_e4m3(qkv, ctx, b, kv)
         return ops.gemm(o, self.out_weight, ctx.act, bias=self.out_bias, partial_sums=True)
 
     def _forward_row_norm(self, normed, ctx, b, kv, amplitude):
