@@ -882,12 +882,18 @@ static int e4m3_cuts(int B, int nh, int max_new, int max_end) {
   const int64_t groups = (int64_t)((max_end + 4 * E4M3_TILE - 1) / (4 * E4M3_TILE)) * nh * B;
   return (int)max((int64_t)1, min((int64_t)(max_new + 255) / 256, 4096 / groups));
 }
+// Whether heads of 16 DT numbers can go through one launch (wider ones: two waves to a SIMD have too few registers), and with how many bytes
+// of shared memory a step up to position max_end does; 0 where it takes two launches and scratch.
+#define SHORT_HEADS(DT) ((DT) <= 12 && (DT) * PIECES <= 24)
+static size_t e4m3_short_bytes(int max_end, int g, int hd) {
+  const size_t shmem = (size_t)((max_end + E4M3_TILE - 1) / E4M3_TILE) * g * (hd + 2) * sizeof(float);
+  return max_end <= SHORT_END && g <= 16 && shmem <= 64 * 1024 ? shmem : 0;
+}
 template <int DT, bool MOD>
 static int launch_decode(const E4m3Attn& a, int max_end, hipStream_t st) {
   const int g = a.nh / a.nkv, columns = a.nkv * ((g + 15) / 16);
-  if constexpr (DT <= 12 && DT * PIECES <= 24) {      // (wider heads: two waves to a SIMD have too few registers)
-    const size_t shmem = (size_t)((max_end + E4M3_TILE - 1) / E4M3_TILE) * g * (a.pages.hd + 2) * sizeof(float);
-    if (max_end <= SHORT_END && g <= 16 && shmem <= 64 * 1024) {
+  if constexpr (SHORT_HEADS(DT)) {
+    if (const size_t shmem = e4m3_short_bytes(max_end, g, a.pages.hd)) {
       hipLaunchKernelGGL((e4m3_short_kernel<DT, MOD>), dim3(columns, a.B), dim3(64 * SHORT_WAVES), shmem, st, a);
       return 0;
     }
@@ -949,6 +955,8 @@ static int launch(const E4m3Attn& a, int decode, int max_new, int max_end, hipSt
 TQ_API int64_t tq_e4m3_attention_scratch(int T, int B, int nh, int nkv, int hd, int max_new, int max_end, int decode, int weights) {
   const int64_t ld = (max_end + E4M3_TILE - 1) / E4M3_TILE * E4M3_TILE;
   if (!decode) return weights ? (int64_t)B * e4m3_cuts(B, nh, max_new, max_end) * nh * ld + (int64_t)T * nh : 0;
+  // (the kernels are made for heads of 4, 8, 12 and 16 times 16 numbers)
+  if (SHORT_HEADS((hd + 63) / 64 * 4) && e4m3_short_bytes(max_end, nh / nkv, hd)) return weights ? (int64_t)B * nh * ld : 0;
   return (int64_t)B * nh * e4m3_most_runs(max_end, nh / nkv) * (hd + 2) + (weights ? (int64_t)B * nh * ld : 0);
 }
 
@@ -962,7 +970,7 @@ TQ_API int tq_e4m3_attention(const void* q, void* out, const int* cu, const int*
   if (B <= 0 || T <= 0) return 0;
   if ((r1 == nullptr) != (r2 == nullptr) || chunk < 0 || softcap < 0.f || window < 0 || nh <= 0 || max_new <= 0 || max_end <= 0) return TQ_ERR_BAD_ARG;
   if (!e4m3_pages_fit(page_size, heads, head0, nkv, hd) || nh % nkv != 0 || nh > 65535 || nh / nkv > 1024 || B > 65535) return TQ_ERR_UNSUPPORTED;
-  if ((decode || weight) && !scratch) return TQ_ERR_BAD_ARG;
+  if (!scratch && tq_e4m3_attention_scratch(T, B, nh, nkv, hd, max_new, max_end, decode, weight != nullptr)) return TQ_ERR_BAD_ARG;
   E4m3Attn a{(const act_t*)q, (act_t*)out, cu, slots, start, B, nh, nkv, window, scale, ScoreMod{softcap, r1, r2, chunk, sink, nullptr, 0},
              nullptr, e4m3_most_runs(max_end, nh / nkv), nullptr, 0, nullptr,
              E4m3Pages{(uint8_t*)k, (uint8_t*)v, (float*)k_scale, (float*)v_scale, weight, table, bt_stride, page_size, heads, head0, hd}};

@@ -1348,7 +1348,7 @@ def attention_writes_into(act, head_dim: int, scale: float) -> bool:
 E4M3_BLOCK = 16      # positions that share a scale
 
 
-@dataclasses.dataclass(frozen=True, eq=False)
+@dataclasses.dataclass(frozen=True, eq=False, init=False)
 class E4m3Pages:
     """Pages of keys and values as e4m3 codes with a scale, a power of two, for each block of 16 positions of a layer's kv head.
 
@@ -1370,23 +1370,34 @@ class E4m3Pages:
     table: torch.Tensor
     weight: torch.Tensor | None = None
 
-    def __post_init__(self):
+    def __init__(self, k, v, k_scale, v_scale, table, weight=None):
         """Checks the pools once, for all calls with these pages."""
-        k, table, w = self.k, self.table, self.weight
-        shape, dev, code = k.shape, k.get_device(), torch.float8_e4m3fn
-        ps = self.k_scale.shape[-1] * E4M3_BLOCK
-        hd = shape[-1] // ps if ps else 0
-        small, at = (*shape[:-1], ps // E4M3_BLOCK), table.shape
-        if not (dev >= 0 and len(shape) == 4 and ps % 64 == 0 and hd % 16 == 0 and 16 <= hd <= 256 and shape[3] == hd * ps and len(at) == 2
-                and _lies(k, code, shape, dev) and _lies(self.v, code, shape, dev) and _lies(self.k_scale, torch.float32, small, dev)
-                and _lies(self.v_scale, torch.float32, small, dev) and _lies(table, torch.int32, at, dev)
-                and (w is None or _lies(w, torch.float32, (*shape[:3], ps), dev)) and k.numel() and not (k.data_ptr() | self.v.data_ptr()) % 16):
+        self.__dict__.update(k=k, v=v, k_scale=k_scale, v_scale=v_scale, table=table, weight=weight)
+        code, f32, good = torch.float8_e4m3fn, torch.float32, False
+        try:      # (one expression, for the sake of the host's time; what is wrong is found out afterwards)
+            shape, small, at, dev = k.shape, k_scale.shape, table.shape, k.get_device()
+            ps = small[-1] * E4M3_BLOCK
+            hd = shape[-1] // ps
+            good = (dev >= 0 and len(shape) == 4 and ps % 64 == 0 and hd % 16 == 0 and 16 <= hd <= 256 and shape[3] == hd * ps
+                    and small[:3] == shape[:3] and v.shape == shape and v_scale.shape == small and len(at) == 2 and len(small) == 4
+                    and k.dtype is code and v.dtype is code and k_scale.dtype is f32 and v_scale.dtype is f32 and table.dtype is torch.int32
+                    and dev == v.get_device() == k_scale.get_device() == v_scale.get_device() == table.get_device()
+                    and k.is_contiguous() and v.is_contiguous() and k_scale.is_contiguous() and v_scale.is_contiguous() and table.is_contiguous()
+                    and (weight is None or (weight.dtype is f32 and weight.shape == (*shape[:3], ps) and weight.get_device() == dev
+                                            and weight.is_contiguous()))
+                    and shape[0] > 0 and shape[1] > 0 and shape[2] > 0 and not (k.data_ptr() | v.data_ptr()) % 16)
+        except (AttributeError, IndexError, ZeroDivisionError):
+            pass
+        if not good:
             self._explain()
         self.__dict__.update(page_size=ps, head_dim=hd, layers=shape[1], num_kv_heads=shape[2], device_index=dev, table_shape=(at[0], at[1]))
 
     def _explain(self):
-        k, shape = "E4m3Pages", self.k.shape
-        _need(len(shape) == 4 and self.k.is_cuda, k, "k must be [pages, layers, kv heads, page_size * head_dim] on the GPU")
+        k = "E4m3Pages"
+        for name in ("k", "v", "k_scale", "v_scale", "table"):
+            _check(getattr(self, name), k, name)
+        shape = self.k.shape
+        _need(len(shape) == 4 and self.k_scale.dim() == 4, k, "k must be [pages, layers, kv heads, page_size * head_dim], its scales as many dimensions")
         ps = self.k_scale.shape[-1] * E4M3_BLOCK
         _need(ps > 0 and ps % 64 == 0, k, lambda: f"pages must hold a multiple of 64 positions, hold {ps}")
         _need(shape[3] % (16 * ps) == 0 and 16 <= shape[3] // ps <= 256, k,
@@ -1478,7 +1489,7 @@ def rope_kv_write_e4m3(qkv: torch.Tensor, positions: torch.Tensor, inv_freq: tor
     _check_here(inv_freq, k, "inv_freq", torch.float32, (rotary_dim // 2,) if rotary_dim else None, dev)
     where, B, max_new, _max_end, _decode = _e4m3_runs(k, runs, pages, T, dev)
     act = dtype_name(act)
-    q = torch.empty((T, num_heads * hd), dtype=ACT_DTYPES[act], device=positions.device)
+    q = qkv.new_empty((T, num_heads * hd), dtype=ACT_DTYPES[act])
     pools = pages._args(layer, True)
     if not write:
         pools = (None, *pools[1:])
@@ -1518,7 +1529,7 @@ def attention_e4m3(q: torch.Tensor, pages: E4m3Pages, layer: int, num_heads: int
     lib = library(act)
     out = torch.empty_like(q)
     n = lib.tq_e4m3_attention_scratch(T, B, num_heads, nkv, hd, max_new, max_end, decode, add_weights) if decode or add_weights else 0
-    scratch = torch.empty((n,), dtype=torch.float32, device=q.device) if n else None
+    scratch = q.new_empty((n,), dtype=torch.float32) if n else None
     _run(k, lib.tq_e4m3_attention(
         q.data_ptr(), out.data_ptr(), *where, T, B, num_heads, nkv, hd, window or 0, scale, softcap or 0.0, _ptr(r1), _ptr(r2), chunk or 0,
         _ptr(sink), *pages._args(layer, add_weights), _ptr(scratch), decode, max_new, max_end, _raw_stream(dev)))
