@@ -78,12 +78,7 @@ __device__ __forceinline__ bf16x8 nothing() {
   return __builtin_bit_cast(bf16x8, w);
 }
 // Eight numbers of a query from dimension d on; zeros behind the head's end and for a column without a query.
-__device__ __forceinline__ void load_query(bf16x8 (&out)[PIECES], const act_t* row, int d, int hd, bool valid) {
-  if (!valid || d >= hd) {
-#pragma unroll
-    for (int p = 0; p < PIECES; ++p) out[p] = nothing();
-    return;
-  }
+__device__ __forceinline__ void load_query(bf16x8 (&out)[PIECES], const act_t* row, int d) {
 #if defined(TQ_ACT_BF16)
   out[0] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(row + d));
 #else
@@ -91,6 +86,11 @@ __device__ __forceinline__ void load_query(bf16x8 (&out)[PIECES], const act_t* r
   const float x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
   pieces_of(x, out);
 #endif
+}
+__device__ __forceinline__ void load_query(bf16x8 (&out)[PIECES], const act_t* row, int d, int hd, bool valid) {
+  if (valid && d < hd) return load_query(out, row, d);
+#pragma unroll
+  for (int p = 0; p < PIECES; ++p) out[p] = nothing();
 }
 __device__ __forceinline__ float group_max(float v) { return with_lane_xor<32>(with_lane_xor<16>(v, LanesMax()), LanesMax()); }
 __device__ __forceinline__ float group_sum(float v) { return with_lane_xor<32>(with_lane_xor<16>(v, LanesSum()), LanesSum()); }
@@ -800,6 +800,12 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DT * PIECES
 #pragma unroll
   for (int jt = 0; jt < 4; ++jt) acc[jt] = f32x4{0.f, 0.f, 0.f, 0.f};
   if (from < to) ask(from);
+  // (a condition at every read would keep the next from being on its way: rows are filled up with zeros once)
+  for (int i = tid; i < 2 * WEIGHT_TOKENS * (DT - hd / 16); i += 256) {
+    act_t* at = qs + i / (DT - hd / 16) * PITCH + hd + i % (DT - hd / 16) * 16;
+#pragma unroll
+    for (int e = 0; e < 16; e += PER) *reinterpret_cast<u32x4*>(at + e) = u32x4{0u, 0u, 0u, 0u};
+  }
   int buf = 0;
   for (int q0 = from; q0 < to; q0 += WEIGHT_TOKENS, buf ^= 1) {
     // (one barrier a round: the buffer that is written was last read before the one before)
@@ -825,7 +831,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DT * PIECES
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
         bf16x8 qf[PIECES];
-        load_query(qf, qrow, 64 * (ks / 2) + 16 * c + 8 * (ks % 2), hd, true);
+        load_query(qf, qrow, 64 * (ks / 2) + 16 * c + 8 * (ks % 2));
 #pragma unroll
         for (int jt = 0; jt < 4; ++jt)
 #pragma unroll
