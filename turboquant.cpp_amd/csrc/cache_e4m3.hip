@@ -595,12 +595,12 @@ TQ_API int tq_e4m3_choose(const int* slots, const int* lengths, int B, int max_l
 
 // ------------------------------------------------------------------------------------------ eviction: the move
 // A workgroup fills one tile of 64 positions of one sequence, layer and kv head from the positions that were chosen, each wherever it
-// lies: keys 16 bytes at a time; values, whose positions lie side by side, by bytes out of the source's tiles, which come through LDS whole,
-// three at a time (positions are in ascending order: a tile of which half the positions stay comes from two or three).  A thread
+// lies: keys 16 bytes at a time; values, whose positions lie side by side, by bytes out of the source's tiles, which come through LDS whole
+// (positions are in ascending order: a tile of which half the positions stay comes from two or three).  A thread
 // puts 16 positions of a dimension together.  A block's scale is the largest of its positions' blocks; the codes of the others are
 // brought to it.  Rows behind the last position are zeros up to the end of their page.
-// Bound by the bytes: lines of the source are read whole, twice what stays where every other position does.
-#define MOVE_TILES 3
+// Bound by the bytes: lines of the source are read whole, twice what stays where every other position does.  Half of 8 sequences of
+// 8,192 positions, 6 layers and 16 kv heads of 128, 1.6 GB read and 0.8 written, take 532 us (a large copy of as many bytes 470).
 #define MOVE_PITCH 80      // bytes between the dimensions of a tile in LDS: 16 of them, four positions each, touch banks of their own
 typedef unsigned int u32x4_t __attribute__((ext_vector_type(4)));
 struct E4m3Move {
@@ -608,11 +608,12 @@ struct E4m3Move {
   const int* dst;
   const int* kept;
   int keep, slots_of_table, tiles;
+  int at_once;                  // tiles of values that come through LDS at a time
   E4m3Pages pages;
 };
 template <int VI>
 __global__ __launch_bounds__(256) void e4m3_move_kernel(E4m3Move a) {
-  extern __shared__ __attribute__((aligned(16))) uint8_t tiles[];      // [3][hd][80]
+  extern __shared__ __attribute__((aligned(16))) uint8_t tiles[];      // [at_once][hd][80]
   __shared__ int from[E4M3_TILE], at_slot[E4M3_TILE], n_slots;      // places in the source; which of its tiles (numbered as they come)
   __shared__ int64_t head_of[E4M3_TILE];
   __shared__ int64_t tile_of[E4M3_TILE];      // where the numbered tiles lie
@@ -675,8 +676,8 @@ __global__ __launch_bounds__(256) void e4m3_move_kernel(E4m3Move a) {
   }
   uint32_t w[2 * VI][4] = {};
   const int slots = n_slots;
-  for (int s0 = 0; s0 < slots; s0 += MOVE_TILES) {
-    const int n = min(MOVE_TILES, slots - s0);
+  for (int s0 = 0; s0 < slots; s0 += a.at_once) {
+    const int n = min(a.at_once, slots - s0);
     if (s0) __syncthreads();
     for (int i = tid; i < n * hd * 4; i += 256)
       *reinterpret_cast<u32x4_t*>(tiles + i / 4 * MOVE_PITCH + i % 4 * 16) =
@@ -727,11 +728,14 @@ TQ_API int tq_e4m3_move(const int* src, const int* dst, int B, const int* kept, 
   if (B <= 0) return 0;
   if (keep < 1) return TQ_ERR_BAD_ARG;
   if (!e4m3_pages_fit(page_size, heads, 0, 1, hd) || keep > (int64_t)bt_stride * page_size) return TQ_ERR_UNSUPPORTED;
-  E4m3Move a{src, dst, kept, keep, slots_of_table, (keep + page_size - 1) / page_size * (page_size / E4M3_TILE),
+  E4m3Move a{src, dst, kept, keep, slots_of_table, (keep + page_size - 1) / page_size * (page_size / E4M3_TILE), 1,
              E4m3Pages{(uint8_t*)k, (uint8_t*)v, k_scale, v_scale, weight, table, bt_stride, page_size, heads, 0, hd}};
   const int64_t groups = (int64_t)a.tiles * heads * B;
   if (groups > 0xFFFFFF) return TQ_ERR_UNSUPPORTED;      // (a launch's threads are counted in 32 bits)
-  const size_t shmem = (size_t)MOVE_TILES * hd * MOVE_PITCH;      // at most 60 KiB
+  // Many workgroups hide one another's waiting, the more the less memory each takes (us of the move above with one, two and three tiles:
+  // 532, 567, 654); few of them wait less often with more tiles (96 of them, one sequence: 9.6, 8.3, 7.9).
+  if (groups <= 2048) a.at_once = 3;
+  const size_t shmem = (size_t)a.at_once * hd * MOVE_PITCH;      // at most 60 KiB
   if (hd <= 128) hipLaunchKernelGGL(e4m3_move_kernel<1>, dim3((unsigned)groups), dim3(256), shmem, st, a);
   else hipLaunchKernelGGL(e4m3_move_kernel<2>, dim3((unsigned)groups), dim3(256), shmem, st, a);
   TQ_LAUNCH_CHECK();
