@@ -411,6 +411,38 @@ def test_move(ops, D, page, keep, lens):
     assert torch.equal(raw[pages.table[:len(lens)].long()], pages.k.view(torch.uint8)[pages.table[:len(lens)].long()])
 
 
+def test_move_of_many_tiles(ops):
+    """Enough workgroups (more than 2,048) that one tile of values at a time goes through shared memory."""
+    lens, keep = [1300, 1217], 650
+    pages, plain = filled(ops, lens, 8, 16, 32, 64, True, slots=4, loud=2.0 ** 30)
+    kept = ops.evict_choose(pages, dev([0, 1]), dev(lens), max(lens), keep, 4, 100)
+    assert -(-keep // 64) * 8 * 16 * 2 > 2048
+    ops.evict_move(pages, dev([0, 1]), dev([2, 3]), kept)
+    got, host = P.read_pages(pages, 32), kept.cpu().numpy()
+    for s in (0, 1):
+        P.move(plain, s, s + 2, host[s], 64)
+    for m in "kv":
+        assert np.array_equal(got.code[m], plain.code[m]) and np.array_equal(got.scale[m], plain.scale[m]), m
+    assert np.array_equal(got.weight, plain.weight)
+
+
+def test_a_bias_from_any_place_on(ops):
+    """Views of a bias that start between multiples of 16 bytes."""
+    pages = make_pages(ops, 1, 20, 1, 2, 32)
+    for dtype in (torch.bfloat16, torch.float32):
+        bias = torch.randn(1 + 8 * 32, dtype=dtype, device=DEV)
+        x, pos, freq = torch.randn(3, 8 * 32, device=DEV), dev([0, 1, 2]), torch.rand(16, device=DEV)
+        q = [ops.rope_kv_write_e4m3(x, pos, freq, 0, 32, pages, 0, 4, "bfloat16", make_runs([0], [0], [3]), bias=b)
+             for b in (bias[1:], bias[1:].clone())]
+        assert torch.equal(*q)
+
+
+def test_short_caches_at_the_most_shared_memory(ops):
+    """14 tiles of 9 heads of 128 to a kv head: 64 bytes more than go through one launch."""
+    check_attention(ops, "bfloat16", 9, 1, 128, [895], [1])
+    check_attention(ops, "bfloat16", 9, 1, 128, [830], [1])
+
+
 def test_move_of_few_positions_and_bad_places(ops):
     """Sequences of fewer positions than are asked for; positions and slots that lie outside are passed over."""
     pages, plain = filled(ops, [40, 150], 1, 1, 32, 64, True, slots=4)

@@ -271,6 +271,19 @@ def test_a_conversation_saved_and_loaded(folders, act, tmp_path):
         model.load_context(path)
         assert model.chat_tokens == history
         assert model.chat(history + [5, 6]) == want
+    from turboquant_cpp_amd.engine.step import Engine
+    with Model(folder, kv_cache="e4m3", **options) as model:      # what each position has received goes along, or starts at nothing
+        weighing = Engine(model._model, 1024, kv_cache="e4m3", track_weights=True)
+        slot = weighing.open(1)[0]
+        weighing.step([slot], [history])
+        saved = weighing.cache.export_slot(slot)
+        again, bare = weighing.cache.import_slot(saved), model.engine.cache.import_slot(saved)
+        for a, b in zip(weighing.cache.export_slot(again)["groups"], saved["groups"]):
+            assert all(torch.equal(a[n], b[n]) for n in ("keys", "values", "key_scales", "value_scales", "weights"))
+        for a, b in zip(model.engine.cache.export_slot(bare)["groups"], saved["groups"]):
+            assert torch.equal(a["keys"], b["keys"]) and "weights" not in a
+        for a in weighing.cache.export_slot(weighing.cache.import_slot(model.engine.cache.export_slot(bare)))["groups"]:
+            assert not a["weights"].any()
     with Model(folder, **options) as model, pytest.raises(RuntimeError, match="another layout"):
         model.load_context(path)
     with Model(folder, **options) as model:

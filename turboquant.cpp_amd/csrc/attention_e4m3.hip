@@ -893,7 +893,7 @@ static int e4m3_cuts(int B, int nh, int max_new, int max_end) {
 #define SHORT_HEADS(DT) ((DT) <= 12 && (DT) * PIECES <= 24)
 static size_t e4m3_short_bytes(int max_end, int g, int hd) {
   const size_t shmem = (size_t)((max_end + E4M3_TILE - 1) / E4M3_TILE) * g * (hd + 2) * sizeof(float);
-  return max_end <= SHORT_END && g <= 16 && shmem <= 64 * 1024 ? shmem : 0;
+  return max_end <= SHORT_END && g <= 16 && shmem + 16 * sizeof(float) <= 64 * 1024 ? shmem : 0;      // (and the heads' sums of 16)
 }
 template <int DT, bool MOD>
 static int launch_decode(const E4m3Attn& a, int max_end, hipStream_t st) {

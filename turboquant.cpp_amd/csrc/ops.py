@@ -1484,6 +1484,8 @@ def rope_kv_write_e4m3(qkv: torch.Tensor, positions: torch.Tensor, inv_freq: tor
           "rows of qkv must have unit stride and start at multiples of 16 bytes")
     if bias is not None:
         _check_here(bias, k, "bias", torch.bfloat16 if bias.dtype is torch.bfloat16 else torch.float32, (width,), dev)
+        if bias.data_ptr() % 16:
+            bias = bias.clone()      # (it is read four numbers at a time)
     _need(0 <= rotary_dim <= hd and rotary_dim % 2 == 0 and (pairing == 0 or pairing == 1), k,
           lambda: f"rotary_dim must be even and at most a head's {hd}, pairing 0 or 1")
     _check_here(inv_freq, k, "inv_freq", torch.float32, (rotary_dim // 2,) if rotary_dim else None, dev)
@@ -1505,7 +1507,8 @@ def attention_e4m3(q: torch.Tensor, pages: E4m3Pages, layer: int, num_heads: int
     """``attention`` over pages of 8 bits: each token attends to its sequence's cached positions up to its own; returns [T, nh * hd].
     Places count here (the runs'), not the positions that keys were rotated by.  The options are ``attention``'s.  ``add_weights``:
     every position's number in ``pages.weight`` is raised by the weights it receives from the step's tokens and the heads of its kv head,
-    exp(score) over the softmax's denominator (sums in a fixed order: the same step gives the same bits).  A row whose scores are
+    exp(score) over the softmax's denominator (sums in a fixed order: the same step gives the same bits; no slot may stand in the runs
+    twice then).  A row whose scores are
     all -inf is 0 and gives no weight."""
     k = "attention_e4m3"
     dev, act = pages._here(k, layer), dtype_name(act)
@@ -1566,8 +1569,8 @@ def evict_choose(pages: E4m3Pages, slots: torch.Tensor, lengths: torch.Tensor, m
 
 def evict_move(pages: E4m3Pages, src_slots: torch.Tensor, dst_slots: torch.Tensor, kept: torch.Tensor, act="bfloat16") -> None:
     """Copies the positions ``kept`` [B, layers, kv heads, keep] (as ``evict_choose`` gives them, in ascending order; -1: none) of the
-    sequences in ``src_slots`` to places 0, 1, .. of ``dst_slots``, keys, values and weights.  The slots' pages must be different ones: nothing
-    is copied in place.  A block's scale becomes the largest of its rows'; what lies behind the last row in its page becomes zero.  A
+    sequences in ``src_slots`` to places 0, 1, .. of ``dst_slots``, keys, values and weights.  The slots' pages must be different ones, and
+    no slot may be filled twice: nothing is copied in place.  A block's scale becomes the largest of its rows'; what lies behind the last row in its page becomes zero.  A
     row of the table that is -1 where a page is written, or a slot outside the table, is passed over."""
     k = "evict_move"
     dev, B = _evict_slots(k, pages, src_slots, "src_slots")
