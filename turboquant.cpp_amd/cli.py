@@ -9,7 +9,7 @@ is the reference's teacher-forced perplexity (/root/reference/tools/quant.c:430-
 report and, with ``--json``, its JSON; ``--save-logits FILE`` and ``--kl-baseline FILE`` go with it as in the reference
 (:542-556, :594-636): the first writes every scored position's probabilities, the second reports the mean KL divergence
 of such a file against this run (the 32-bit path against the bfloat16 path, for instance, or a cache in 8 bits,
-``--kv-cache e4m3``, against one that is not).  ``--save-kv FILE`` and
+``--kv-cache e4m3``, against one that is not; ``--when-full evict`` lets half of a full sequence's positions go there).  ``--save-kv FILE`` and
 ``--load-kv FILE`` are the reference's too (/root/reference/src/engine/tq_generate.c:268-362): the cache of one prompt
 saved once it has run, and a later run that starts from it with its prompt behind the saved tokens.
 """
