@@ -77,7 +77,7 @@ __device__ __forceinline__ bf16x8 nothing() {
   const u32x4 w = {0u, 0u, 0u, 0u};
   return __builtin_bit_cast(bf16x8, w);
 }
-// Eight numbers of a query from dimension d on; zeros behind the head's end and for a column without a query.
+// Eight numbers of a query from dimension d on.
 __device__ __forceinline__ void load_query(bf16x8 (&out)[PIECES], const act_t* row, int d) {
 #if defined(TQ_ACT_BF16)
   out[0] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(row + d));
@@ -87,10 +87,15 @@ __device__ __forceinline__ void load_query(bf16x8 (&out)[PIECES], const act_t* r
   pieces_of(x, out);
 #endif
 }
+// The same, and zeros behind the head's end and for a column without a query (whose row is some other's: a read without a condition does not
+// keep the next from being on its way).
 __device__ __forceinline__ void load_query(bf16x8 (&out)[PIECES], const act_t* row, int d, int hd, bool valid) {
-  if (valid && d < hd) return load_query(out, row, d);
+  load_query(out, row, min(d, hd - 8));
 #pragma unroll
-  for (int p = 0; p < PIECES; ++p) out[p] = nothing();
+  for (int p = 0; p < PIECES; ++p) {
+    const u32x4 w = __builtin_bit_cast(u32x4, out[p]), none = {0u, 0u, 0u, 0u};
+    out[p] = __builtin_bit_cast(bf16x8, valid && d < hd ? w : none);
+  }
 }
 __device__ __forceinline__ float group_max(float v) { return with_lane_xor<32>(with_lane_xor<16>(v, LanesMax()), LanesMax()); }
 __device__ __forceinline__ float group_sum(float v) { return with_lane_xor<32>(with_lane_xor<16>(v, LanesSum()), LanesSum()); }
@@ -222,7 +227,7 @@ struct DecodeWave {
   float m, l;
 
   __device__ __forceinline__ DecodeWave(const E4m3Attn& args, int b, int kv, int cg) : a(args), kvh(kv) {
-    const int lane = threadIdx.x % 64, g = a.nh / a.nkv, hd = a.pages.hd;
+    const int lane = threadIdx.x % 64, g = a.nh / a.nkv;
     r = lane % 16;
     c = lane / 16;
     p = a.start[b];
@@ -233,12 +238,16 @@ struct DecodeWave {
     r1 = MOD && a.mod.r1 ? a.mod.r1[h] : 0.f;
     r2 = MOD && a.mod.r1 ? a.mod.r2[h] : 0.f;
     ch = change_of(a);
+    clear();
+  }
+  // (behind the first tile's codes, which are then on their way)
+  __device__ __forceinline__ void take_query(int b) {
+    const int hd = a.pages.hd;
     const act_t* qrow = a.q + ((int64_t)a.cu[b] * a.nh + h) * hd;
 #pragma unroll
     for (int s = 0; s < DT / 4; ++s)
 #pragma unroll
       for (int half = 0; half < 2; ++half) load_query(qf[2 * s + half], qrow, 64 * s + 16 * c + 8 * half, hd, valid);
-    clear();
   }
   __device__ __forceinline__ void clear() {
 #pragma unroll
@@ -457,6 +466,7 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(DT > 12 || D
   float* out = a.partial + ((int64_t)b * a.nh + w.h) * a.max_runs * (a.pages.hd + 2);
   w.fetch_k(beg);
   w.fetch_v(beg);
+  w.take_query(b);
   for (int tile = beg; tile < end; ++tile) {
     w.step(b, tile, tile + 1 < end ? tile + 1 : -1);
     if ((tile + 1) % S == 0 || tile + 1 == end) w.leave(out + (int64_t)(tile / S) * (a.pages.hd + 2));
@@ -509,6 +519,7 @@ __global__ __launch_bounds__(64 * SHORT_WAVES) __attribute__((amdgpu_waves_per_e
     w.fetch_k(beg + wave);
     w.fetch_v(beg + wave);
   }
+  w.take_query(b);
   for (int tile = beg + wave; tile < end; tile += SHORT_WAVES) {
     w.step(b, tile, tile + SHORT_WAVES < end ? tile + SHORT_WAVES : -1);
     w.leave(sums + ((tile - beg) * heads + min(w.r, heads - 1)) * stride);
@@ -554,24 +565,6 @@ __global__ __launch_bounds__(256 * HALVES) __attribute__((amdgpu_waves_per_eu(DT
   const int* row = a.pages.table + (int64_t)a.slots[b] * a.pages.bt_stride;
   const float r1 = MOD && a.mod.r1 ? a.mod.r1[h] : 0.f, r2 = MOD && a.mod.r1 ? a.mod.r2[h] : 0.f;
   const Change ch = change_of(a);
-  bf16x8 qf[QG][KS][PIECES];
-  f32x4 o[QG][DT];
-  float m[QG], l[QG];
-  int p[QG], lo[QG];
-#pragma unroll
-  for (int g = 0; g < QG; ++g) {
-    const int qi = qb + (wave * QG + g) * 16 + r;
-    const bool valid = qi < n;
-    p[g] = valid ? start + qi : -1;
-    lo[g] = reach_lo(p[g], a.window, a.mod.chunk);
-    const act_t* qrow = a.q + ((int64_t)(t0 + (valid ? qi : 0)) * a.nh + h) * hd;
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) load_query(qf[g][ks], qrow, 32 * ks + 8 * c, hd, valid);
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt) o[g][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
-    m[g] = a.mod.sink && half == 0 ? a.mod.sink[h] * LOG2E : -INFINITY;
-    l[g] = m[g] != -INFINITY && c == 0 ? 1.f : 0.f;      // (the sink counts once)
-  }
   const int wg_last = start + min(qb + 64 * QG, n) - 1;
   const int tile_beg = reach_lo(start + qb, a.window, a.mod.chunk) / E4M3_TILE, tile_end = wg_last / E4M3_TILE + 1;
   const int wq0 = qb + wave * 16 * QG;
@@ -613,15 +606,33 @@ __global__ __launch_bounds__(256 * HALVES) __attribute__((amdgpu_waves_per_eu(DT
       }
     }
   };
+  const int tile0 = tile_beg + half;
+  if (tile0 < tile_end) fetch_tile(tile0);      // (on its way while the queries are)
+  bf16x8 qf[QG][KS][PIECES];
+  f32x4 o[QG][DT];
+  float m[QG], l[QG];
+  int p[QG], lo[QG];
+#pragma unroll
+  for (int g = 0; g < QG; ++g) {
+    const int qi = qb + (wave * QG + g) * 16 + r;
+    const bool valid = qi < n;
+    p[g] = valid ? start + qi : -1;
+    lo[g] = reach_lo(p[g], a.window, a.mod.chunk);
+    const act_t* qrow = a.q + ((int64_t)(t0 + (valid ? qi : 0)) * a.nh + h) * hd;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) load_query(qf[g][ks], qrow, 32 * ks + 8 * c, hd, valid);
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) o[g][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    m[g] = a.mod.sink && half == 0 ? a.mod.sink[h] * LOG2E : -INFINITY;
+    l[g] = m[g] != -INFINITY && c == 0 ? 1.f : 0.f;      // (the sink counts once)
+  }
   __bf16* mine = tiles + half * 2 * BUF;
   // what lies behind a head's end in LDS is read against zeros of the queries (keys) or not stored (values): it has to be finite
   if (hd < 16 * DT) {
     for (int i = tid; i < 2 * BUF / 8; i += 256) *reinterpret_cast<bf16x8*>(mine + 8 * i) = nothing();
     __syncthreads();
   }
-  const int tile0 = tile_beg + half;
   if (tile0 < tile_end) {
-    fetch_tile(tile0);
     stage(mine);
     if (tile0 + HALVES < tile_end) fetch_tile(tile0 + HALVES);
   }
@@ -928,7 +939,8 @@ static int launch_as(const E4m3Attn& a, int decode, int max_new, int max_end, hi
   if (decode) return launch_decode<DT, MOD>(a, max_end, st);
   // Two groups of 16 tokens to a wave halve the reads from LDS, and the chip does 733 TFLOP/s instead of 505 (8,192 tokens of 16 heads of
   // 128), but it takes enough workgroups that the last blocks, which see most, do not stand alone: 2,048 tokens, 256 of
-  // them, take 47 us so and 42 with one group; 4,096 tokens, 512 of them, 101 and 136.
+  // them, take 47 us so and 42 with one group; 4,096 tokens, 512 of them, 101 and 136.  (These and the next were timed in turn before the
+  // first tile was asked for ahead of the queries, which takes some 2 us off each: the 42 are 40 now.)
   constexpr int TWO = PIECES == 1 && DT <= 8 ? 2 : 1, HALVES = DT <= 8 ? 2 : 1;
   const int64_t of_two = (int64_t)((max_new + 127) / 128) * a.nh * a.B, of_one = (int64_t)((max_new + 63) / 64) * a.nh * a.B;
   const bool two = TWO == 2 && of_two > 256;
