@@ -586,9 +586,10 @@ TQ_API int tq_e4m3_choose(const int* slots, const int* lengths, int B, int max_l
   E4m3Choice a{slots, lengths, kept, keep, first, recent, slots_of_table, max_length,
                E4m3Pages{nullptr, nullptr, nullptr, nullptr, (float*)weight, table, bt_stride, page_size, heads, 0, 16}};
   const size_t shmem = (size_t)(max_length < CHOICE_HELD ? max_length : CHOICE_HELD) * 4;
-  // (always the most: another thread's launch may come between)
-  const hipError_t e = hipFuncSetAttribute((const void*)e4m3_choice_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, CHOICE_HELD * 4);
-  if (e != hipSuccess) return (int)e;
+  if (shmem > 56 * 1024) {      // (with what the kernel has beside it more than goes unasked; always the most: another thread's launch may come between)
+    const hipError_t e = hipFuncSetAttribute((const void*)e4m3_choice_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, CHOICE_HELD * 4);
+    if (e != hipSuccess) return (int)e;
+  }
   hipLaunchKernelGGL(e4m3_choice_kernel, dim3(heads, B), dim3(1024), shmem, st, a);
   TQ_LAUNCH_CHECK();
   return 0;
