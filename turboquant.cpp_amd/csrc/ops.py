@@ -1390,7 +1390,8 @@ class E4m3Pages:
             pass
         if not good:
             self._explain()
-        self.__dict__.update(page_size=ps, head_dim=hd, layers=shape[1], num_kv_heads=shape[2], device_index=dev, table_shape=(at[0], at[1]))
+        self.__dict__.update(page_size=ps, head_dim=hd, layers=shape[1], num_kv_heads=shape[2], device_index=dev, table_shape=(at[0], at[1]),
+                             reach=at[1] * ps, heads=shape[1] * shape[2])
 
     def _explain(self):
         k = "E4m3Pages"
@@ -1424,13 +1425,15 @@ class E4m3Pages:
     def _args(self, layer: int, weight: bool) -> tuple:
         return (self.k.data_ptr(), self.v.data_ptr(), self.k_scale.data_ptr(), self.v_scale.data_ptr(),
                 self.weight.data_ptr() if weight and self.weight is not None else None, self.table.data_ptr(), self.table_shape[1],
-                self.page_size, self.layers * self.num_kv_heads, layer * self.num_kv_heads)
+                self.page_size, self.heads, layer * self.num_kv_heads)
 
-    def _here(self, k: str, layer: int = 0) -> int:
-        """The pages' device, which has to be the current one; whether they have that layer."""
+    def _here(self, layer: int = 0) -> bool:
+        """Whether the pages' device is the current one, and they have that layer."""
+        return self.device_index == torch.cuda.current_device() and 0 <= layer < self.layers
+
+    def _explain_here(self, k: str, layer: int = 0) -> None:
         _need(self.device_index == torch.cuda.current_device(), k, lambda: f"the pages lie on GPU {self.device_index}, which is not the current device")
         _need(0 <= layer < self.layers, k, lambda: f"layer {layer} is none of the pages' {self.layers}")
-        return self.device_index
 
 
 def _lies(t: torch.Tensor, dtype, shape, device: int) -> bool:
@@ -1445,19 +1448,24 @@ def _check_here(t: torch.Tensor, kernel: str, name: str, dtype, shape, device: i
         raise KernelError(f"{kernel}: {name} lies on {t.device}, the other tensors on GPU {device}")
 
 
-def _e4m3_runs(k: str, runs: dict, pages: E4m3Pages, T: int, dev: int):
-    cu, slots, start = runs["cu_seqlens"], runs["slots"], runs["start"]
-    B = slots.numel()
-    if not (_lies(cu, torch.int32, (B + 1,), dev) and _lies(slots, torch.int32, (B,), dev) and _lies(start, torch.int32, (B,), dev)):
-        _check_here(cu, k, "cu_seqlens", torch.int32, (B + 1,), dev)
-        _check_here(slots, k, "slots", torch.int32, (B,), dev)
-        _check_here(start, k, "start", torch.int32, (B,), dev)
-    max_new, max_end, decode = int(runs["max_new"]), int(runs["max_end"]), bool(runs["decode"])
-    if 0 < max_end <= pages.table_shape[1] * pages.page_size and 1 <= max_new <= T and B <= T and (not decode or (T == B and max_new == 1)):
-        return (cu.data_ptr(), slots.data_ptr(), start.data_ptr()), B, max_new, max_end, decode
-    _need(0 < max_end <= pages.table_shape[1] * pages.page_size, k, "positions reach beyond the page table")
-    _need(1 <= max_new <= T and B <= T, k, "the runs do not fit the tokens")
-    raise KernelError(f"{k}: decoding brings one token per sequence")
+def _e4m3_runs(runs: dict, pages: E4m3Pages, T: int, dev: int):
+    """What the kernels are told of the runs, or None where something is wrong with them."""
+    cu, slots, start, max_new, max_end, decode = runs["cu_seqlens"], runs["slots"], runs["start"], runs["max_new"], runs["max_end"], runs["decode"]
+    B, i32 = slots.numel(), torch.int32
+    if (cu.dtype is i32 and slots.dtype is i32 and start.dtype is i32 and cu.shape == (B + 1,) and slots.dim() == 1 and start.shape == (B,)
+            and dev == cu.get_device() == slots.get_device() == start.get_device() and cu.is_contiguous() and slots.is_contiguous()
+            and start.is_contiguous() and 0 < max_end <= pages.reach and 1 <= max_new <= T and B <= T and (not decode or (T == B and max_new == 1))):
+        return cu.data_ptr(), slots.data_ptr(), start.data_ptr(), B, int(max_new), int(max_end), bool(decode)
+    return None
+
+
+def _explain_runs(k: str, runs: dict, pages: E4m3Pages, T: int, dev: int) -> None:
+    B = runs["slots"].numel()
+    for name, n in (("cu_seqlens", B + 1), ("slots", B), ("start", B)):
+        _check_here(runs[name], k, name, torch.int32, (n,), dev)
+    _need(0 < runs["max_end"] <= pages.reach, k, "positions reach beyond the page table")
+    _need(1 <= runs["max_new"] <= T and B <= T, k, "the runs do not fit the tokens")
+    _need(not runs["decode"] or (T == B and runs["max_new"] == 1), k, "decoding brings one token per sequence")
 
 
 def rope_kv_write_e4m3(qkv: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, pairing: int, rotary_dim: int,
@@ -1470,34 +1478,42 @@ def rope_kv_write_e4m3(qkv: torch.Tensor, positions: torch.Tensor, inv_freq: tor
     start at zero.  ``write`` False: the queries alone, for a layer that reads another layer's cache (``qkv`` then holds no keys
     and values)."""
     k = "rope_kv_write_e4m3"
-    dev, T = pages._here(k, layer), positions.numel()
-    nkv, hd = pages.num_kv_heads if write else 0, pages.head_dim
+    dev, T = pages.device_index, positions.numel()
+    nkv, hd, f32 = pages.num_kv_heads if write else 0, pages.head_dim, torch.float32
     width = (num_heads + 2 * nkv) * hd
-    _need(num_heads >= 1 and T >= 1, k, "there must be a head and a token")
-    _check_here(positions, k, "positions", torch.int32, (T,), dev)
-    _need(isinstance(qkv, torch.Tensor) and qkv.get_device() == dev and qkv.dtype is torch.float32 and qkv.shape == (T, width), k,
-          lambda: f"qkv must be float32 [{T}, {width}] on GPU {dev}")
+    at = _e4m3_runs(runs, pages, T, dev)
+    # (one expression, for the sake of the host's time; what is wrong is found out afterwards)
+    if not (at is not None and pages._here(layer) and num_heads >= 1 and positions.dtype is torch.int32 and positions.dim() == 1
+            and positions.get_device() == dev and positions.is_contiguous() and qkv.dtype is f32 and qkv.shape == (T, width)
+            and qkv.get_device() == dev and (bias is None or (bias.dtype in _WTYPE and bias.shape == (width,) and bias.get_device() == dev and bias.is_contiguous()))
+            and 0 <= rotary_dim <= hd and rotary_dim % 2 == 0 and (pairing == 0 or pairing == 1) and inv_freq.dtype is f32
+            and (inv_freq.shape == (rotary_dim // 2,) or rotary_dim == 0) and inv_freq.get_device() == dev and inv_freq.is_contiguous()):
+        pages._explain_here(k, layer)
+        _need(num_heads >= 1 and T >= 1, k, "there must be a head and a token")
+        _check_here(positions, k, "positions", torch.int32, (T,), dev)
+        _need(qkv.get_device() == dev and qkv.dtype is f32 and qkv.shape == (T, width), k, f"qkv must be float32 [{T}, {width}] on GPU {dev}")
+        if bias is not None:
+            _check_here(bias, k, "bias", torch.bfloat16 if bias.dtype is torch.bfloat16 else f32, (width,), dev)
+        _need(0 <= rotary_dim <= hd and rotary_dim % 2 == 0 and pairing in (0, 1), k, f"rotary_dim must be even and at most a head's {hd}, pairing 0 or 1")
+        _check_here(inv_freq, k, "inv_freq", f32, (rotary_dim // 2,) if rotary_dim else None, dev)
+        _explain_runs(k, runs, pages, T, dev)
     ld, one = qkv.stride()
     if T == 1:
         ld = width
-    _need(one == 1 and ld >= width and ld % 4 == 0 and qkv.data_ptr() % 16 == 0, k,
-          "rows of qkv must have unit stride and start at multiples of 16 bytes")
-    if bias is not None:
-        _check_here(bias, k, "bias", torch.bfloat16 if bias.dtype is torch.bfloat16 else torch.float32, (width,), dev)
-        if bias.data_ptr() % 16:
-            bias = bias.clone()      # (it is read four numbers at a time)
-    _need(0 <= rotary_dim <= hd and rotary_dim % 2 == 0 and (pairing == 0 or pairing == 1), k,
-          lambda: f"rotary_dim must be even and at most a head's {hd}, pairing 0 or 1")
-    _check_here(inv_freq, k, "inv_freq", torch.float32, (rotary_dim // 2,) if rotary_dim else None, dev)
-    where, B, max_new, _max_end, _decode = _e4m3_runs(k, runs, pages, T, dev)
+    x = qkv.data_ptr()
+    if one != 1 or ld < width or ld % 4 or x % 16:
+        raise KernelError(f"{k}: rows of qkv must have unit stride and start at multiples of 16 bytes")
+    if bias is not None and bias.data_ptr() % 16:
+        bias = bias.clone()      # (it is read four numbers at a time)
     act = dtype_name(act)
     q = qkv.new_empty((T, num_heads * hd), dtype=ACT_DTYPES[act])
     pools = pages._args(layer, True)
     if not write:
         pools = (None, *pools[1:])
+    cu, slots, start, B, max_new, _max_end, _decode = at
     _run(k, library(act).tq_e4m3_write(
-        qkv.data_ptr(), ld, _ptr(bias), 0 if bias is None else _WTYPE[bias.dtype], positions.data_ptr(), inv_freq.data_ptr(), pairing, rotary_dim,
-        amplitude, *where, q.data_ptr(), T, B, max_new, num_heads, nkv, hd, *pools, _raw_stream(dev)))
+        x, ld, _ptr(bias), 0 if bias is None else _WTYPE[bias.dtype], positions.data_ptr(), inv_freq.data_ptr(), pairing, rotary_dim,
+        amplitude, cu, slots, start, q.data_ptr(), T, B, max_new, num_heads, nkv, hd, *pools, _raw_stream(dev)))
     return q
 
 
@@ -1511,39 +1527,45 @@ def attention_e4m3(q: torch.Tensor, pages: E4m3Pages, layer: int, num_heads: int
     twice then).  A row whose scores are
     all -inf is 0 and gives no weight."""
     k = "attention_e4m3"
-    dev, act = pages._here(k, layer), dtype_name(act)
-    _need(isinstance(q, torch.Tensor) and q.dim() == 2, k, "q must be [T, heads * head_dim]")
+    dev, act = pages.device_index, dtype_name(act)
     T, nkv, hd = q.shape[0], pages.num_kv_heads, pages.head_dim
-    _need(T >= 1 and num_heads >= 1 and num_heads % nkv == 0, k, "heads must be a multiple of kv heads, and there must be a token")
-    _check_here(q, k, "q", ACT_DTYPES[act], (T, num_heads * hd), dev)
-    _need(q.data_ptr() % 16 == 0, k, "q must start at a multiple of 16 bytes")
-    _need(math.isfinite(scale), k, "scale must be finite")
-    _need((window is None or window >= 1) and (chunk is None or chunk >= 1) and (softcap is None or 0 < softcap < math.inf), k,
-          "window, chunk and softcap must be positive")
-    r1 = r2 = None
-    if distance_bias is not None:
-        r1, r2 = distance_bias
-        _check_here(r1, k, "r1", torch.float32, (num_heads,), dev)
-        _check_here(r2, k, "r2", torch.float32, (num_heads,), dev)
-    if sink is not None:
-        _check_here(sink, k, "sink", torch.float32, (num_heads,), dev)
-    _need(not add_weights or pages.weight is not None, k, "these pages keep no weights")
-    where, B, max_new, max_end, decode = _e4m3_runs(k, runs, pages, T, dev)
+    at = _e4m3_runs(runs, pages, T, dev)
+    r1, r2 = (None, None) if distance_bias is None else distance_bias
+    if not (at is not None and pages._here(layer) and num_heads >= 1 and num_heads % nkv == 0 and q.dtype is ACT_DTYPES[act]
+            and q.shape == (T, num_heads * hd) and q.get_device() == dev and q.is_contiguous() and q.data_ptr() % 16 == 0 and math.isfinite(scale)
+            and (window is None or window >= 1) and (chunk is None or chunk >= 1) and (softcap is None or 0 < softcap < math.inf)
+            and (r1 is None or (_lies(r1, torch.float32, (num_heads,), dev) and _lies(r2, torch.float32, (num_heads,), dev)))
+            and (sink is None or _lies(sink, torch.float32, (num_heads,), dev)) and (not add_weights or pages.weight is not None)):
+        pages._explain_here(k, layer)
+        _need(T >= 1 and num_heads >= 1 and num_heads % nkv == 0, k, "heads must be a multiple of kv heads, and there must be a token")
+        _check_here(q, k, "q", ACT_DTYPES[act], (T, num_heads * hd), dev)
+        _need(q.data_ptr() % 16 == 0, k, "q must start at a multiple of 16 bytes")
+        _need(math.isfinite(scale), k, "scale must be finite")
+        _need((window is None or window >= 1) and (chunk is None or chunk >= 1) and (softcap is None or 0 < softcap < math.inf), k,
+              "window, chunk and softcap must be positive")
+        for name, t in (("r1", r1), ("r2", r2), ("sink", sink)):
+            if t is not None or (name == "r2" and r1 is not None):
+                _check_here(t, k, name, torch.float32, (num_heads,), dev)
+        _need(not add_weights or pages.weight is not None, k, "these pages keep no weights")
+        _explain_runs(k, runs, pages, T, dev)
+    cu, slots, start, B, max_new, max_end, decode = at
     lib = library(act)
     out = torch.empty_like(q)
     n = lib.tq_e4m3_attention_scratch(T, B, num_heads, nkv, hd, max_new, max_end, decode, add_weights) if decode or add_weights else 0
     scratch = q.new_empty((n,), dtype=torch.float32) if n else None
     _run(k, lib.tq_e4m3_attention(
-        q.data_ptr(), out.data_ptr(), *where, T, B, num_heads, nkv, hd, window or 0, scale, softcap or 0.0, _ptr(r1), _ptr(r2), chunk or 0,
+        q.data_ptr(), out.data_ptr(), cu, slots, start, T, B, num_heads, nkv, hd, window or 0, scale, softcap or 0.0, _ptr(r1), _ptr(r2), chunk or 0,
         _ptr(sink), *pages._args(layer, add_weights), _ptr(scratch), decode, max_new, max_end, _raw_stream(dev)))
     return out
 
 
-def _evict_slots(k: str, pages: E4m3Pages, slots: torch.Tensor, name: str) -> tuple[int, int]:
-    dev = pages._here(k)
-    _need(isinstance(slots, torch.Tensor) and slots.dim() == 1, k, lambda: f"{name} must be [B]")
-    B = slots.numel()
-    _check_here(slots, k, name, torch.int32, (B,), dev)
+def _evict_slots(k: str, pages: E4m3Pages, one: torch.Tensor, other: torch.Tensor) -> tuple[int, int]:
+    """The pages' device and how many sequences the two int32 tensors [B] are about."""
+    dev, B = pages.device_index, one.numel()
+    if not (pages._here() and _lies(one, torch.int32, (B,), dev) and _lies(other, torch.int32, (B,), dev)):
+        pages._explain_here(k)
+        for t in (one, other):
+            _check_here(t, k, "every list of sequences", torch.int32, (B,), dev)
     return dev, B
 
 
@@ -1554,31 +1576,29 @@ def evict_choose(pages: E4m3Pages, slots: torch.Tensor, lengths: torch.Tensor, m
     in all; of equal weights the lower position stays, and NaN counts as the largest.  int32 [B, layers, kv heads, keep] in ascending
     order.  A sequence of ``keep`` positions or fewer keeps them all, with -1 behind them."""
     k = "evict_choose"
-    dev, B = _evict_slots(k, pages, slots, "slots")
-    _check_here(lengths, k, "lengths", torch.int32, (B,), dev)
+    dev, B = _evict_slots(k, pages, slots, lengths)
     _need(pages.weight is not None, k, "these pages keep no weights")
-    _need(keep >= 1 and first >= 0 and recent >= 0 and first + recent <= keep, k,
-          lambda: f"the first {first} and last {recent} positions must lie within the {keep} that stay")
-    _need(0 <= max_length <= pages.table_shape[1] * pages.page_size, k, "positions reach beyond the page table")
-    kept = torch.empty((B, pages.layers, pages.num_kv_heads, keep), dtype=torch.int32, device=slots.device)
+    if not (keep >= 1 and first >= 0 and recent >= 0 and first + recent <= keep):
+        raise KernelError(f"{k}: the first {first} and last {recent} positions must lie within the {keep} that stay")
+    _need(0 <= max_length <= pages.reach, k, "positions reach beyond the page table")
+    kept = slots.new_empty((B, pages.layers, pages.num_kv_heads, keep))
     _run(k, library(act).tq_e4m3_choose(slots.data_ptr(), lengths.data_ptr(), B, max_length, keep, first, recent, kept.data_ptr(),
                                         pages.weight.data_ptr(), pages.table.data_ptr(), *pages.table_shape, pages.page_size,
-                                        pages.layers * pages.num_kv_heads, _raw_stream(dev)))
+                                        pages.heads, _raw_stream(dev)))
     return kept
 
 
 def evict_move(pages: E4m3Pages, src_slots: torch.Tensor, dst_slots: torch.Tensor, kept: torch.Tensor, act="bfloat16") -> None:
     """Copies the positions ``kept`` [B, layers, kv heads, keep] (as ``evict_choose`` gives them, in ascending order; -1: none) of the
     sequences in ``src_slots`` to places 0, 1, .. of ``dst_slots``, keys, values and weights.  The slots' pages must be different ones, and
-    no slot may be filled twice: nothing is copied in place.  A block's scale becomes the largest of its rows'; what lies behind the last row in its page becomes zero.  A
-    row of the table that is -1 where a page is written, or a slot outside the table, is passed over."""
+    no slot may be filled twice: nothing is copied in place.  A block's scale becomes the largest of its rows'; what lies behind the
+    last row in its page becomes zero.  A row of the table that is -1 where a page is written, or a slot outside the table, is passed over."""
     k = "evict_move"
-    dev, B = _evict_slots(k, pages, src_slots, "src_slots")
-    _check_here(dst_slots, k, "dst_slots", torch.int32, (B,), dev)
+    dev, B = _evict_slots(k, pages, src_slots, dst_slots)
     _need(isinstance(kept, torch.Tensor) and kept.dim() == 4 and kept.shape[3] >= 1, k, "kept must be [B, layers, kv heads, keep]")
     keep = kept.shape[3]
     _check_here(kept, k, "kept", torch.int32, (B, pages.layers, pages.num_kv_heads, keep), dev)
-    _need(keep <= pages.table_shape[1] * pages.page_size, k, "positions reach beyond the page table")
+    _need(keep <= pages.reach, k, "positions reach beyond the page table")
     pools = pages._args(0, True)
     _run(k, library(act).tq_e4m3_move(src_slots.data_ptr(), dst_slots.data_ptr(), B, kept.data_ptr(), keep, pages.head_dim, *pools[:6],
                                       *pages.table_shape, *pools[7:9], _raw_stream(dev)))
