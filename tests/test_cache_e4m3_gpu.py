@@ -426,6 +426,25 @@ def test_move_of_many_tiles(ops):
     assert np.array_equal(got.weight, plain.weight)
 
 
+@pytest.mark.parametrize("step", [0, 1, 3, -2])
+def test_positions_that_do_not_follow_one_another(ops, step):
+    """What a run's tokens turn by is what `positions` says, one by one: steps of any size, and now and then another."""
+    T, D, rng = 150, 128, np.random.RandomState(abs(step))
+    pages, freq = make_pages(ops, 1, T, 1, 2, D), torch.tensor(10000.0 ** (-np.arange(64) / 64), dtype=torch.float32)
+    at = 70_000 + step * np.arange(T) + np.cumsum(rng.rand(T) < 0.05) * 11
+    x = torch.randn(T, 8 * D, generator=torch.Generator().manual_seed(1))
+    q = ops.rope_kv_write_e4m3(x.to(DEV), dev(at.tolist()), freq.to(DEV), 0, D, pages, 0, 4, "float32", make_runs([0], [0], [T]))
+    x = x.double().numpy().reshape(T, 8, D)
+    want, length = P.rotate(x[:, :4], at, freq.double().numpy(), 0), np.hypot(x[:, :4, :64], x[:, :4, 64:])
+    off = np.abs(q.cpu().double().numpy().reshape(T, 4, D) - want)
+    assert (off <= 2.0 ** -21 * np.concatenate([length, length], -1)).all()
+    k = P.rotate(x[:, 4:6], at, freq.double().numpy(), 0)
+    got = P.read_pages(pages, D)
+    for h in range(2):
+        held, scale = got.values("k", 0, 0, h)[:T], got.scale["k"][0, 0, h].repeat(P.BLOCK)[:T, None]
+        assert (np.abs(held - k[:, h]) <= (2.0 ** -4 + 2.0 ** -20) * np.abs(k[:, h]) + 2.0 ** -10 * scale + 2.0 ** -20 * np.abs(k[:, h]).max()).all()
+
+
 def test_a_bias_from_any_place_on(ops):
     """Views of a bias that start between multiples of 16 bytes."""
     pages = make_pages(ops, 1, 20, 1, 2, 32)
