@@ -851,11 +851,24 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DT * PIECES
       const float sum = lses[buf][16 * half + r];
       // every token of the 16 sees the whole tile: nothing to compare
       const bool masked = q1 + 15 >= n || start + q1 < pos0 + E4M3_TILE - 1 || reach_lo(start + q1 + 15, a.window, a.mod.chunk) > pos0;
-      final_scores<MOD>(s, a, ch, r1, r2, pos0, p, lo, masked);
+      final_scores<MOD>(s, a, ch, r1, r2, pos0, p, lo, false);
 #pragma unroll
       for (int jt = 0; jt < 4; ++jt)
 #pragma unroll
-        for (int v = 0; v < 4; ++v) acc[jt][v] += __builtin_amdgcn_exp2f(fmaf(s[jt][v], MOD ? 1.f : ch.scale2, -sum));
+        for (int v = 0; v < 4; ++v) s[jt][v] = __builtin_amdgcn_exp2f(fmaf(s[jt][v], MOD ? 1.f : ch.scale2, -sum));
+      // (by its place, not by a score of -inf: the sum of a row that is not a number is none either, and would reach positions it does not see)
+      if (masked) {
+        asm volatile("");      // (a branch, as in final_scores)
+#pragma unroll
+        for (int jt = 0; jt < 4; ++jt)
+#pragma unroll
+          for (int v = 0; v < 4; ++v) {
+            const int key = pos0 + 16 * jt + 4 * c + v;
+            s[jt][v] = key <= p && key >= lo ? s[jt][v] : 0.f;
+          }
+      }
+#pragma unroll
+      for (int jt = 0; jt < 4; ++jt) acc[jt] += s[jt];
     }
   }
   if (!has) return;

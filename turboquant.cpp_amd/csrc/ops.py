@@ -1525,7 +1525,7 @@ def attention_e4m3(q: torch.Tensor, pages: E4m3Pages, layer: int, num_heads: int
     every position's number in ``pages.weight`` is raised by the weights it receives from the step's tokens and the heads of its kv head,
     exp(score) over the softmax's denominator (sums in a fixed order: the same step gives the same bits; no slot may stand in the runs
     twice then).  A row whose scores are
-    all -inf is 0 and gives no weight."""
+    all -inf is 0 and gives no weight; one whose sum is not a number gives NaN to the positions that it sees, and nothing to any other."""
     k = "attention_e4m3"
     dev, act = pages.device_index, dtype_name(act)
     T, nkv, hd = q.shape[0], pages.num_kv_heads, pages.head_dim
