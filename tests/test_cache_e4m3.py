@@ -289,3 +289,15 @@ def test_pages_of_another_device_than_the_current_one(pretend, monkeypatch):
     with pytest.raises(ops.KernelError, match="not the current device"):
         ops.attention_e4m3(torch.zeros(1, 128, dtype=torch.bfloat16), pages, 0, 4, None, 1.0, "bfloat16", runs_of((0,), (1,)))
     assert not pretend.calls
+
+
+def test_a_sequence_that_has_let_positions_go_is_not_continued_by_its_history():
+    """Its length is not the number of tokens that it has seen."""
+    from turboquant_cpp_amd.engine.generate import continue_in_slot
+    c = cache_of(need(), tokens=64 * 6, max_slots=2)
+    slot = grown(c, 200)
+    c.begin_evict(slot, 70)
+    c.end_evict(slot, 70)
+    engine = types.SimpleNamespace(cache=c, length=c.length)
+    with pytest.raises(CacheError, match="let positions go"):
+        continue_in_slot(engine, slot, list(range(100)) * 3)

@@ -418,3 +418,29 @@ def test_designs_against_their_pages_in_the_activations_type(monkeypatch, tmp_pa
         assert max(errs) < 1e-4, f"row {int(np.argmax(errs))} of {len(errs)} differs by {max(errs):.2e}"
     else:
         assert np.median(errs) < 0.06 and np.quantile(errs, 0.9) < 0.12, (np.median(errs), np.quantile(errs, 0.9))
+
+
+def test_a_conversation_that_has_let_positions_go(folders, tmp_path):
+    """Its cache is not what it has seen: it starts over, cannot be continued in its slot, and is not saved."""
+    from turboquant_cpp_amd import Model
+    from turboquant_cpp_amd.cache.paged import CacheError
+    from turboquant_cpp_amd.engine.generate import continue_in_slot
+    folder, _plain = folders("A", "bfloat16")
+    V = DENSE["A"]["vocab_size"]
+    history, path = tokens(V, 100, 1), str(tmp_path / "kv.safetensors")
+    with Model(folder, kv_cache="e4m3", when_full="evict", temperature=0.0, stop_tokens=[], max_tokens=6, context_length=256, max_batch=2) as model:
+        want = model.chat(history + [5, 6])
+        for again in (history + [5, 6], history + [5, 6] + want):
+            model.reset_chat()
+            model.feed(history)
+            model.engine.evict([model._chat_slot], 50)
+            with pytest.raises(RuntimeError, match="let positions go"):
+                model.save_context(path)
+            with pytest.raises(CacheError, match="let positions go"):
+                continue_in_slot(model.engine, model._chat_slot, again)
+            fed = model.feed(again)
+            assert fed == len(again) and model.engine.cache.slots[model._chat_slot].dropped == 0
+            model.reset_chat()
+            model.feed(history)
+            model.engine.evict([model._chat_slot], 50)
+            assert model.chat(history + [5, 6]) == want

@@ -118,7 +118,8 @@ class Model:
         run again, only the rest is, and the continuation comes back.  ``None`` ends the conversation, as
         ``reset_chat``.  Where the history parts from what the cache holds, the cache goes back to that point if it
         can (no window has dropped pages there), else the conversation starts over.  Raises
-        :class:`ChatContextOverflow` (and resets) when the history does not fit the context."""
+        :class:`ChatContextOverflow` (and resets) when the history does not fit the context.  A conversation whose slot has
+        let positions go (``Engine.evict``) starts over too."""
         self._ensure_open()
         if history is None:
             self.reset_chat()
@@ -152,8 +153,8 @@ class Model:
 
     @property
     def chat_tokens(self) -> list[int]:
-        """The tokens that the conversation's cache holds."""
-        if self._chat_slot is None:
+        """The tokens that the conversation's cache holds (none, if it has let positions go: they are not the first ones)."""
+        if self._chat_slot is None or self._engine.cache.dropped(self._chat_slot):
             return []
         return self._chat_tokens[:self._engine.length(self._chat_slot)]
 
@@ -169,6 +170,9 @@ class Model:
             raise ChatContextOverflow("conversation history exceeds the model's context window; the session has "
                                       "been reset, retry with a shorter history")
         if self._chat_slot is None:
+            self._chat_slot, self._chat_tokens = eng.open(1)[0], []
+        if eng.cache.dropped(self._chat_slot):      # what it holds is no beginning of anything
+            eng.close([self._chat_slot])
             self._chat_slot, self._chat_tokens = eng.open(1)[0], []
         held = self._chat_tokens[:eng.length(self._chat_slot)]
         limit = min(len(held), len(history) - (1 if keep_last else 0))
@@ -196,6 +200,8 @@ class Model:
         self._ensure_open()
         if self._chat_slot is None:
             raise RuntimeError("there is no conversation to save")
+        if self._engine.cache.dropped(self._chat_slot):
+            raise RuntimeError("the conversation has let positions go: its cache does not hold its first tokens")
         from .weights.safetensors_io import write_safetensors
         data = self._engine.cache.export_slot(self._chat_slot)
         tensors = {"tokens": torch.tensor(self._chat_tokens[:data["length"]], dtype=torch.int32)}

@@ -478,6 +478,10 @@ class PagedCache:
             return "layers with a window or chunks count on the places of all positions"
         return None
 
+    def dropped(self, slot: int) -> int:
+        """How many positions of its sequence have been let go."""
+        return self._live(slot).dropped
+
     def positions_of(self, slots, places) -> list[int]:
         """The positions of tokens at these places of the slots' sequences."""
         return [p + self.slots[s].dropped for s, p in zip(slots, places)]

@@ -23,7 +23,7 @@ from typing import Callable, Sequence
 
 import torch
 
-from ..cache.paged import CacheFull
+from ..cache.paged import CacheError, CacheFull
 from ..sampling.sampler import Sampler, SamplingOptions, TokenFetch
 
 
@@ -266,9 +266,12 @@ def continue_in_slot(engine, slot: int, history: Sequence[int], options: Generat
     """One sequence that outlives the call, as the reference's chat keeps its state between turns
     (/root/reference/quant.h:17634-17700): ``history`` is everything the sequence has seen and is to see, the slot's
     cache holds its first ``engine.length(slot)`` tokens (fewer than all of them), the rest is run as one prompt step
-    and a continuation is generated.  Nothing is let go: the history is what the cache holds.  The slot stays open; afterwards its cache holds the history and the generated
+    and a continuation is generated.  Nothing is let go: the history is what the cache holds, and a slot that has let
+    positions go is refused (CacheError).  The slot stays open; afterwards its cache holds the history and the generated
     tokens but the last, if that one ended the turn by its number (``engine.length(slot)`` says how many)."""
     o = options or GenerationOptions()
+    if engine.cache.dropped(slot):
+        raise CacheError(f"slot {slot} has let positions go: its length does not say what of the history it has seen")
     cached = engine.length(slot)
     if not 0 <= cached < len(history):
         raise ValueError(f"the cache holds {cached} tokens, the history {len(history)}: at least one must be new")
