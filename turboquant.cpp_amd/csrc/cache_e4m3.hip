@@ -375,16 +375,20 @@ __global__ __launch_bounds__(WRITE_THREADS) __attribute__((amdgpu_waves_per_eu(K
   }
 }
 
-// One new token to a sequence: a wave takes a head of queries, or a kv head's key and value, four neighbouring numbers a lane, and the
-// waves of a workgroup share the token's cosines and sines.  The same roundings as above.  Bound by the reads that follow one another
+// One new token to a sequence, or none: a wave takes a head of a row's queries, or the key and value of a kv head of a sequence's token, four
+// neighbouring numbers a lane, and the waves of a workgroup, which do the one or the other, share the token's cosines and sines.  (Rows of queries
+// are as many as sequences, and taken by themselves: where a sequence brings no token there are rows that belong to none.)  The same roundings
+// as above.  Bound by the reads that follow one another
 // and by fetching the code: 8 tokens of 16 heads of 128 on 16 take 5.0 us, and 10.2 in the kernel above, whose code is many times as long.
 template <bool FOURS>
 __global__ __launch_bounds__(256) void e4m3_write_one_kernel(E4m3Write a) {
   extern __shared__ __attribute__((aligned(16))) float2 turns[];
-  const int hd = a.hd, n = a.rot / 2, b = blockIdx.y, t = a.cu[b], lane = threadIdx.x % 64;
-  const int h = (int)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x / 64), kvh = h - a.nh;
-  if (a.cu[b + 1] == t) return;
-  const bool mine = h < a.nh + (a.write ? a.nkv : 0), keys = kvh >= 0, has = 4 * lane < hd;
+  const int hd = a.hd, n = a.rot / 2, b = blockIdx.y, lane = threadIdx.x % 64, of_queries = (a.nh + 3) / 4;
+  const bool keys = (int)blockIdx.x >= of_queries;
+  const int t = keys ? a.cu[b] : b;
+  if (keys && a.cu[b + 1] == t) return;
+  const int kvh = ((int)blockIdx.x - of_queries) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x / 64), h = keys ? a.nh + kvh : kvh + of_queries * 4;
+  const bool mine = h < (keys ? a.nh + a.nkv : a.nh), has = 4 * lane < hd;
   const int d = has ? 4 * lane : 0, col = mine ? h * hd : 0, vcol = mine && keys ? col + a.nkv * hd : col;
   const float* base = a.x + (int64_t)t * a.ld;
   Raw raw = read_four<FOURS>(a, base, 0, col, d);
@@ -469,8 +473,8 @@ TQ_API int tq_e4m3_write(const float* x, int64_t ld, const void* bias, int bias_
   const size_t shmem = (size_t)(a.write ? min(E4M3_TILE, max(max_new, a.q_tokens)) : a.q_tokens) * (rot / 2) * sizeof(float2);      // at most 64 KiB
   const dim3 grid((unsigned)groups), block(WRITE_THREADS);
   const bool fours = rot % (pairing == 0 ? 8 : 4) == 0;
-  if (max_new == 1 && T == B && T <= 65535) {      // (T > B: rows that belong to no sequence have queries too)
-    const dim3 one((nh + (k ? nkv : 0) + 3) / 4, T);
+  if (max_new == 1 && T == B && T <= 65535) {
+    const dim3 one((nh + 3) / 4 + (k ? (nkv + 3) / 4 : 0), T);
     if (fours) hipLaunchKernelGGL(e4m3_write_one_kernel<true>, one, dim3(256), rot / 2 * sizeof(float2), st, a);
     else hipLaunchKernelGGL(e4m3_write_one_kernel<false>, one, dim3(256), rot / 2 * sizeof(float2), st, a);
     TQ_LAUNCH_CHECK();

@@ -1474,8 +1474,8 @@ def rope_kv_write_e4m3(qkv: torch.Tensor, positions: torch.Tensor, inv_freq: tor
     """``rope_kv_write`` into pages of 8 bits: rotates queries and keys, returns the queries [T, nh * hd] and writes keys and values
     of layer ``layer`` as codes.  ``positions`` [T] are what the rotation turns by (the product of position and frequency is taken
     exactly, not rounded to 32 bits first); the places in the cache are the runs' (``start`` and on), which differ from them where a
-    sequence has let positions go.  ``runs`` as for ``attention``; no slot may stand in it twice.  The new places' weights
-    start at zero.  ``write`` False: the queries alone, for a layer that reads another layer's cache (``qkv`` then holds no keys
+    sequence has let positions go.  ``runs`` as for ``attention``; no slot may stand in it twice.  A sequence
+    may bring no token, and a row that belongs to none has its queries all the same.  The new places' weights start at zero.  ``write`` False: the queries alone, for a layer that reads another layer's cache (``qkv`` then holds no keys
     and values)."""
     k = "rope_kv_write_e4m3"
     dev, T = pages.device_index, positions.numel()
