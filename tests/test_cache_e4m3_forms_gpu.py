@@ -77,3 +77,19 @@ def test_queries_of_rows_behind_the_last_sequence(ops, act, cu, rotary):
         assert np.array_equal(got.scale[m], want.scale[m])
         assert_codes(got.code[m], want.code[m])
     assert np.array_equal(got.weight, want.weight)
+
+
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("cu", [[0, 1, 2, 2], [0, 1, 1, 2], [0, 0, 0, 1]])
+@pytest.mark.parametrize("lens", [[300, 70, 5], [1500, 70, 2100], [4200, 1100, 900]])
+def test_single_tokens_beside_sequences_that_bring_none(ops, act, cu, lens):
+    """Those change neither an output nor a weight."""
+    first, _plain = filled(ops, lens, 2, 2, 64, weights=True)
+    second = ops.E4m3Pages(first.k, first.v, first.k_scale, first.v_scale, first.table, first.weight.clone())
+    q = torch.randn((3, 4 * 64), generator=torch.Generator().manual_seed(2)).to(adt(act)).to(DEV)
+    got = ops.attention_e4m3(q, first, 1, 4, None, 0.125, act, padded(cu, [0, 1, 2], [n - 1 for n in lens]), add_weights=True)
+    for b in range(3):
+        if cu[b + 1] > cu[b]:
+            want = ops.attention_e4m3(q[cu[b]:cu[b] + 1].contiguous(), second, 1, 4, None, 0.125, act, make_runs([b], [lens[b] - 1], [1]), add_weights=True)
+            assert torch.equal(got[cu[b]], want[0])
+    assert torch.equal(first.weight, second.weight)

@@ -190,7 +190,7 @@ __device__ __forceinline__ float over(float l) { return l == 0.f ? 0.f : 1.0f / 
 __device__ __forceinline__ float lse_of(float m, float l) { return l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l); }
 
 // ------------------------------------------------------------------------------------------ single tokens
-// One new token per sequence.  A wave takes tiles for up to 16 of the g heads of a kv head, run by run, and leaves a run's unnormalised
+// One new token per sequence, or none.  A wave takes tiles for up to 16 of the g heads of a kv head, run by run, and leaves a run's unnormalised
 // sums, maximum and denominator; the runs are then joined in order.  How the tiles are cut into runs depends on the token's own
 // position and on g only, so a token's result does not depend on what else the step holds.  Up to SHORT_END positions a workgroup does
 // it all, its waves' runs meeting in LDS: one launch.  Beyond, a wave streams through as many runs as make some thousands of
@@ -460,7 +460,7 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(DT > 12 || D
   const int p = a.start[b], S = e4m3_tiles_per_run(p, g), lo = reach_lo(p, a.window, a.mod.chunk);
   const int first_run = lo / E4M3_TILE / S, n_runs = e4m3_runs_at(p, g) - first_run, each = (n_runs + (int)gridDim.x - 1) / (int)gridDim.x;
   const int run0 = first_run + (int)blockIdx.x * each, run1 = min(run0 + each, first_run + n_runs);
-  if (run0 >= run1) return;
+  if (run0 >= run1 || a.cu[b + 1] == a.cu[b]) return;
   DecodeWave<DT, MOD> w(a, b, blockIdx.y / ngc, blockIdx.y % ngc);
   const int beg = max(run0 * S, lo / E4M3_TILE), end = min(run1 * S, p / E4M3_TILE + 1);
   float* out = a.partial + ((int64_t)b * a.nh + w.h) * a.max_runs * (a.pages.hd + 2);
@@ -484,6 +484,7 @@ __global__ __launch_bounds__(256) void e4m3_join_kernel(E4m3Attn a, int blocks_o
   const int b = joins ? x / a.nh : x / blocks_of_weights / a.nkv;
   const int p = a.start[b], lo = reach_lo(p, a.window, a.mod.chunk), S = e4m3_tiles_per_run(p, g);
   const int beg = lo / E4M3_TILE / S, end = p / E4M3_TILE / S + 1;
+  if (a.cu[b + 1] == a.cu[b]) return;
   if (joins) {
     const int h = x % a.nh;
     join_runs<true, E>(a, a.partial + ((int64_t)b * a.nh + h) * a.max_runs * stride, stride, beg, end, h, a.cu[b], wave, lds);
@@ -515,6 +516,7 @@ __global__ __launch_bounds__(64 * SHORT_WAVES) __attribute__((amdgpu_waves_per_e
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64, stride = a.pages.hd + 2, heads = min(16, g - 16 * cg);
   DecodeWave<DT, MOD> w(a, b, kvh, cg);
   const int beg = w.lo / E4M3_TILE, end = w.p / E4M3_TILE + 1;
+  if (a.cu[b + 1] == a.cu[b]) return;
   if (beg + wave < end) {
     w.fetch_k(beg + wave);
     w.fetch_v(beg + wave);
@@ -992,7 +994,7 @@ TQ_API int64_t tq_e4m3_attention_scratch(int T, int B, int nh, int nkv, int hd, 
 }
 
 // q, out [T][nh][hd]; tokens as runs (cu, slots, start) whose keys and values the cache holds already.  decode != 0: one token per
-// sequence.  weight (null: none): every position's is raised by what it receives.  max_end: the largest position + 1.
+// sequence, or none.  weight (null: none): every position's is raised by what it receives.  max_end: the largest position + 1.
 TQ_API int tq_e4m3_attention(const void* q, void* out, const int* cu, const int* slots, const int* start, int T, int B, int nh, int nkv,
                              int hd, int window, float scale, float softcap, const float* r1, const float* r2, int chunk,
                              const float* sink, const void* k, const void* v, const float* k_scale, const float* v_scale, float* weight,

@@ -1521,7 +1521,8 @@ def attention_e4m3(q: torch.Tensor, pages: E4m3Pages, layer: int, num_heads: int
                    softcap: float | None = None, distance_bias: tuple[torch.Tensor, torch.Tensor] | None = None,
                    chunk: int | None = None, sink: torch.Tensor | None = None, add_weights: bool = False) -> torch.Tensor:
     """``attention`` over pages of 8 bits: each token attends to its sequence's cached positions up to its own; returns [T, nh * hd].
-    Places count here (the runs'), not the positions that keys were rotated by.  The options are ``attention``'s.  ``add_weights``:
+    Places count here (the runs'), not the positions that keys were rotated by.  A sequence may bring no token, in a step of single tokens too:
+    it changes nothing, and what stands in a row that belongs to no sequence means nothing.  The options are ``attention``'s.  ``add_weights``:
     every position's number in ``pages.weight`` is raised by the weights it receives from the step's tokens and the heads of its kv head,
     exp(score) over the softmax's denominator (sums in a fixed order: the same step gives the same bits; no slot may stand in the runs
     twice then).  A row whose scores are
