@@ -1,4 +1,5 @@
-"""The 8-bit cache's kernels where rows and runs hold nothing or no numbers."""
+"""The 8-bit cache's kernels where rows and runs hold nothing or no numbers, and at the sizes by which their forms are chosen, against plain
+64-bit arithmetic (plain_e4m3.py) with the tolerances that test_cache_e4m3_gpu.py derives."""
 import math
 
 import numpy as np
@@ -6,7 +7,7 @@ import pytest
 import torch
 
 import plain_e4m3 as P
-from test_cache_e4m3_gpu import ACTS, DEV, adt, dev, filled, make_pages, make_runs, ops  # noqa: F401
+from test_cache_e4m3_gpu import ACTS, DEV, adt, check_write, dev, filled, make_pages, make_runs, ops  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -93,3 +94,11 @@ def test_single_tokens_beside_sequences_that_bring_none(ops, act, cu, lens):
             want = ops.attention_e4m3(q[cu[b]:cu[b] + 1].contiguous(), second, 1, 4, None, 0.125, act, make_runs([b], [lens[b] - 1], [1]), add_weights=True)
             assert torch.equal(got[cu[b]], want[0])
     assert torch.equal(first.weight, second.weight)
+
+
+# ------------------------------------------------------------------------------------------------ writes
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("rotary,pairing", [(256, 0), (256, 1), (254, 0), (254, 1)])
+def test_writes_at_the_most_shared_memory(ops, act, rotary, pairing):
+    """The angles of 64 rows of heads of 256: 64 KiB, and what the kernel has beside them."""
+    check_write(ops, act, 1, 1, 256, rotary, pairing, False, 64, [([0], [64]), ([0], [3]), ([0], [130])])

@@ -470,7 +470,8 @@ TQ_API int tq_e4m3_write(const float* x, int64_t ld, const void* bias, int bias_
   const int64_t kv_groups = a.write ? (int64_t)a.tiles * ((nkv + a.kv_heads - 1) / a.kv_heads) * B : 0;
   const int64_t groups = kv_groups + (int64_t)((T + a.q_tokens - 1) / a.q_tokens) * ((nh + a.q_heads - 1) / a.q_heads);
   if (groups > 0x7FFFFF) return TQ_ERR_UNSUPPORTED;      // (a launch's threads are counted in 32 bits)
-  const size_t shmem = (size_t)(a.write ? min(E4M3_TILE, max(max_new, a.q_tokens)) : a.q_tokens) * (rot / 2) * sizeof(float2);      // at most 64 KiB
+  // at most 64 KiB for the angles of 64 rows of 256 numbers, and the kernel has less than 1 KiB beside them
+  const size_t shmem = (size_t)(a.write ? min(E4M3_TILE, max(max_new, a.q_tokens)) : a.q_tokens) * (rot / 2) * sizeof(float2);
   const dim3 grid((unsigned)groups), block(WRITE_THREADS);
   const bool fours = rot % (pairing == 0 ? 8 : 4) == 0;
   if (max_new == 1 && T == B && T <= 65535) {
@@ -480,10 +481,12 @@ TQ_API int tq_e4m3_write(const float* x, int64_t ld, const void* bias, int bias_
     TQ_LAUNCH_CHECK();
     return 0;
   }
-  if (hd <= 128 && fours) hipLaunchKernelGGL((e4m3_write_kernel<4, true>), grid, block, shmem, st, a);
-  else if (hd <= 128) hipLaunchKernelGGL((e4m3_write_kernel<4, false>), grid, block, shmem, st, a);
-  else if (fours) hipLaunchKernelGGL((e4m3_write_kernel<8, true>), grid, block, shmem, st, a);
-  else hipLaunchKernelGGL((e4m3_write_kernel<8, false>), grid, block, shmem, st, a);
+  const auto kernel = hd <= 128 ? (fours ? e4m3_write_kernel<4, true> : e4m3_write_kernel<4, false>) : fours ? e4m3_write_kernel<8, true> : e4m3_write_kernel<8, false>;
+  if (shmem > 63 * 1024) {      // (with what the kernel has beside it more than goes unasked)
+    const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, 64 * 1024);
+    if (e != hipSuccess) return (int)e;
+  }
+  hipLaunchKernelGGL(kernel, grid, block, shmem, st, a);
   TQ_LAUNCH_CHECK();
   return 0;
 }
