@@ -102,3 +102,41 @@ def test_single_tokens_beside_sequences_that_bring_none(ops, act, cu, lens):
 def test_writes_at_the_most_shared_memory(ops, act, rotary, pairing):
     """The angles of 64 rows of heads of 256: 64 KiB, and what the kernel has beside them."""
     check_write(ops, act, 1, 1, 256, rotary, pairing, False, 64, [([0], [64]), ([0], [3]), ([0], [130])])
+
+
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("T", [1030, 2050, 4099])
+def test_queries_of_several_tokens_to_a_workgroup(ops, act, T):
+    """Two, four and eight of them; positions that follow one another, and some that do not."""
+    nh, D, rotary = 3, 32, 24
+    pages, rng = make_pages(ops, 1, T, 1, 1, D), np.random.RandomState(T)
+    inv = (1e4 ** (-torch.arange(rotary // 2, dtype=torch.float64) / (rotary // 2))).float()
+    at = 50_000 + np.arange(T) + np.cumsum(rng.rand(T) < 0.1) * 13
+    x = torch.randn((T, nh * D), generator=torch.Generator().manual_seed(4))
+    for pairing in (0, 1):
+        q = ops.rope_kv_write_e4m3(x.to(DEV), dev(at.tolist()), inv.to(DEV), pairing, rotary, pages, 0, nh, act, make_runs([0], [0], [T]), write=False)
+        want = P.rotate(x.double().numpy().reshape(T, nh, D), at, inv.double().numpy(), pairing)
+        off = np.abs(q.double().cpu().numpy().reshape(T, nh, D) - want)
+        assert (off <= 2.0 ** -21 * np.abs(x.numpy()).max() + (np.abs(want) * 2.0 ** -8 if act == "bfloat16" else 0.0)).all()
+
+
+@pytest.mark.parametrize("step", [0, 1, 3, -2])
+@pytest.mark.parametrize("start", [0, 37])
+def test_codes_of_keys_whose_positions_do_not_follow_one_another(ops, step, start):
+    """Whole tiles and parts of tiles: the codes of 64-bit angles, but for the few keys that lie next to a border between two."""
+    T, D, rng = 300, 128, np.random.RandomState(abs(step))
+    pages, freq = make_pages(ops, 1, start + T, 1, 2, D), torch.tensor(10000.0 ** (-np.arange(64) / 64), dtype=torch.float32)
+    plain = P.PlainPages(1, 1, 2, D, pages.table.shape[1] * 64)
+    at = 70_000 + step * np.arange(T) + np.cumsum(rng.rand(T) < 0.05) * 11
+    x = torch.randn(T, 5 * D, generator=torch.Generator().manual_seed(1))
+    full = x.double().numpy().reshape(T, 5, D)
+    turned = P.rotate(full[:, 1:3], at, freq.double().numpy(), 0)
+    if start:
+        k, v = rng.randn(start, 2, D), rng.randn(start, 2, D)
+        plain.write(0, 0, 0, k, v)
+        P.fill_pages(pages, plain, D)
+    ops.rope_kv_write_e4m3(x.to(DEV), dev(at.tolist()), freq.to(DEV), 0, D, pages, 0, 1, "float32", make_runs([0], [start], [T]))
+    plain.write(0, 0, start, turned, full[:, 3:])
+    got = P.read_pages(pages, D)
+    assert np.array_equal(got.scale["k"], plain.scale["k"]) and np.array_equal(got.code["v"], plain.code["v"])
+    assert_codes(got.code["k"], plain.code["k"])

@@ -55,20 +55,20 @@ __device__ __forceinline__ float2 turn_of(int p, float f, float amp) {
   const Turn t = turn_at((double)p * (double)f);
   return make_float2(amp * (float)t.c, amp * (float)t.s);
 }
-// The cosines and sines of `rows` tokens, [rows][n], by all threads.  A thread's rows whose positions follow one another take them from the
-// first's by the sum of two angles, four operations instead of some forty, in 64 bits, at most TURN_ROWS - 1 times: off by 2^-29, as the series
-// are (4,096 tokens of 28 heads on 4 31.5 -> 26.9 us, of 16 on 16 39.4 -> 37.2).  A thread with fewer than four rows works each out.
-// MANY: the workgroup may have as many as 64 rows, or few, which then ask for no other positions (32-bit tokens of 1 to 333: 11.2 -> 10.0);
-// with the few of queries all are asked for at once, without a condition (28 heads on 4: 30.8 -> 26.9).
+// The cosines and sines of a tile's `rows` new tokens, [rows][n], by all threads.  A thread's rows whose positions follow one another take them from
+// the first's by the sum of two angles, four operations instead of some forty, in 64 bits: at most TURN_ROWS - 1 times, each of which adds the
+// step's error to what there is, so that they are off by 8 times what the series are at most, 2^-30.  A thread with fewer than four rows works each
+// out, and asks for no other positions.  Against each worked out: 4,096 tokens of 16 heads on 16 45.4 -> 41.1 us, of 28 on 4 33.7 -> 32.6, ragged turns
+// of 3 to 900 51.4 -> 50.6; but 8 turns of 40 to 300 15.2 -> 16.0 and 32-bit ones of 1 to 333 10.3 -> 10.5, whose tiles are mostly new in part.  (Tiles
+// that are new in part by a loop of their own: those 15.2 and 10.4, but the long prompt 42.9.)
 #define TURN_ROWS 8
-template <bool MANY>
 __device__ __forceinline__ void turns_of(const E4m3Write& a, const int* positions, int rows, int n, float2* turns) {
   const int share = min(TURN_ROWS, rows * n / WRITE_THREADS), each = share < 4 ? 1 : share, parts = (rows + each - 1) / each;
   for (int i = threadIdx.x; i < parts * n; i += WRITE_THREADS) {
     const int f = i % n, r0 = i / n * each, count = min(each, rows - r0), p0 = positions[r0];
     const double freq = (double)a.inv_freq[f];
     bool follow = true;
-    if (!MANY || count > 1)
+    if (count > 1)
 #pragma unroll
       for (int u = 1; u < TURN_ROWS; ++u) follow = follow && positions[r0 + min(u, count - 1)] == p0 + min(u, count - 1);
     Turn t = turn_at((double)p0 * freq), step = t;
@@ -153,18 +153,23 @@ __global__ __launch_bounds__(WRITE_THREADS) __attribute__((amdgpu_waves_per_eu(K
     const int w = (int)blockIdx.x - kv_groups, per = (a.nh + a.q_heads - 1) / a.q_heads;
     const int t0 = w / per * a.q_tokens, h0 = w % per * a.q_heads;
     const int nt = min(a.q_tokens, a.T - t0), heads = min(a.q_heads, a.nh - h0);
-    turns_of<false>(a, a.positions + t0, nt, n, turns);
-    __syncthreads();
-    // four items of a thread are on their way at a time
+    // four items of a thread are on their way at a time, the first of them while the angles are worked out (4,096 tokens of 28 heads: 32.6 -> 29.2 us);
+    // a workgroup's few rows give a thread an angle or two, so that no sum of angles would be shared
     const int items = nt * heads * fours;
     const float* base = a.x + (int64_t)t0 * a.ld;
-    for (int i0 = tid; i0 < items; i0 += 4 * WRITE_THREADS) {
-      Raw raw[4];
+    Raw raw[4];
+    auto ask = [&](int i0) {
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         const int i = min(i0 + u * WRITE_THREADS, items - 1), d = i % fours * 4, th = i / fours;
         raw[u] = read_four<FOURS>(a, base, (uint32_t)(th / heads) * ld, (h0 + th % heads) * hd, d);
       }
+    };
+    ask(tid);
+    for (int i = tid; i < nt * n; i += WRITE_THREADS) turns[i] = turn_of(a.positions[t0 + i / n], a.inv_freq[i % n], a.amp);
+    __syncthreads();
+    for (int i0 = tid; i0 < items; i0 += 4 * WRITE_THREADS) {
+      if (i0 != tid) ask(i0);
       if (a.bias)
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
@@ -219,7 +224,7 @@ __global__ __launch_bounds__(WRITE_THREADS) __attribute__((amdgpu_waves_per_eu(K
   const int64_t head0 = e4m3_head_of(a.pages, a.pages.table + (int64_t)a.slots[b] * a.pages.bt_stride, tile, kvh0, in_page);
   if (head0 < 0) return;
   ask_values(kvh0);      // (on their way while the angles are worked out)
-  turns_of<true>(a, a.positions + first + r0, r1 - r0, n, turns);
+  turns_of(a, a.positions + first + r0, r1 - r0, n, turns);
   __syncthreads();
 #pragma unroll 1
   for (int hi = 0; hi < a.kv_heads && kvh0 + hi < a.nkv; ++hi) {
