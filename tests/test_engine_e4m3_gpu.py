@@ -444,3 +444,16 @@ def test_a_conversation_that_has_let_positions_go(folders, tmp_path):
             model.feed(history)
             model.engine.evict([model._chat_slot], 50)
             assert model.chat(history + [5, 6]) == want
+
+
+def test_whose_turn_it_is_to_end_where_nothing_is_free(folders):
+    """Two sequences need pages at once, one to let positions go and the other to grow: the longer one ends, its pages let the other go on."""
+    from turboquant_cpp_amd.engine.generate import GenerationOptions, generate
+    folder, _plain = folders("A", "bfloat16")
+    engine = engine_of(folder, "bfloat16", max_tokens=192, weights=True, max_slots=2, max_positions=100)
+    V = engine.vocab_size
+    options = GenerationOptions(max_tokens=20, temperature=0.0, rep_penalty=1.0, loop_detection=False, max_batch=2, when_full="evict")
+    got = generate(engine, [tokens(V, 99, 1), tokens(V, 63, 2)], options)
+    assert [r.finish_reason for r in got] == ["context", "length"] and [len(r.tokens) for r in got] == [2, 20]
+    got = generate(engine, [tokens(V, 63, 2), tokens(V, 99, 1)], options)
+    assert [r.finish_reason for r in got] == ["length", "context"]

@@ -248,7 +248,8 @@ def generate(engine, prompts: Sequence[Sequence[int]], options: GenerationOption
                         except CacheFull:
                             # the pages have run out: of the sequences that need one, the longest ends here, and
                             # what it held lets the others go on
-                            needy = [i for i in going if engine.cache.needs_page(slot_of[live[i]], 1)]
+                            # (one that holds all it may needs pages for what it is to keep)
+                            needy = [i for i in going if engine.length(slot_of[live[i]]) >= max_pos or engine.cache.needs_page(slot_of[live[i]], 1)]
                             i = max(needy or going, key=lambda i: engine.length(slot_of[live[i]]))
                             going.remove(i)
                             end(live[i], tracks, slot_of, "context")
