@@ -7,7 +7,7 @@ import pytest
 import torch
 
 import plain_e4m3 as P
-from test_cache_e4m3_gpu import ACTS, DEV, adt, check_write, dev, filled, make_pages, make_runs, ops  # noqa: F401
+from test_cache_e4m3_gpu import ACTS, DEV, adt, check_attention, check_write, dev, filled, make_pages, make_runs, ops  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -96,12 +96,166 @@ def test_single_tokens_beside_sequences_that_bring_none(ops, act, cu, lens):
     assert torch.equal(first.weight, second.weight)
 
 
+# ------------------------------------------------------------------------------------------------ prompts whose tiles go to two halves of a workgroup
+HALVES = [
+    (4, 2, 64, [577], [577], dict()),                              # ten tiles, no past
+    (4, 4, 128, [513], [70], dict()),                              # nine tiles, the last of one position
+    (2, 1, 80, [640, 50, 700], [200, 50, 1], dict()),              # heads narrower than their kernel's, a sequence without tiles for one half
+    (3, 3, 48, [530], [129], dict()),
+    (2, 2, 64, [900, 513], [300, 17], dict(window=448)),
+    (2, 1, 64, [650], [650], dict(window=500, sink=True)),
+    (4, 2, 80, [600], [90], dict(sink=True)),
+    (4, 2, 64, [700], [257], dict(softcap=5.0)),
+    (2, 1, 128, [580], [100], dict(bias=True, sink=True)),
+    (2, 2, 64, [640], [200], dict(chunk=300)),
+    (2, 1, 16, [1100], [64], dict(softcap=4.0, sink=True, window=600, bias=True, chunk=1000)),
+]
+
+
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("nh,G,D,lens,new,opts", HALVES)
+def test_prompts_in_two_halves(ops, act, nh, G, D, lens, new, opts):
+    """At most 512 workgroups and at least 512 positions in reach; one group of 16 tokens to a wave."""
+    assert -(-max(new) // 64) * nh * len(new) <= 512 and -(-max(new) // 128) * nh * len(new) <= 256
+    assert min(max(lens), opts.get("window", 10 ** 6) + 64) >= 512
+    check_attention(ops, act, nh, G, D, lens, new, weights=True, **opts)
+
+
+@pytest.mark.parametrize("nh,G,D,lens,new,opts", [(96, 1, 64, [640], [260], dict()), (130, 2, 128, [570], [135], dict(sink=True)),
+                                                  (100, 1, 80, [515], [257], dict(softcap=5.0)), (90, 1, 48, [700], [257], dict(window=450, bias=True))])
+def test_prompts_in_two_halves_with_two_groups(ops, nh, G, D, lens, new, opts):
+    """The same with two groups of 16 tokens to a wave."""
+    assert 256 < -(-max(new) // 128) * nh <= 512
+    check_attention(ops, "bfloat16", nh, G, D, lens, new, weights=True, **opts)
+
+
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("odd", [0, 1])
+def test_halves_whose_scores_are_all_minus_infinity(ops, act, odd):
+    """Every second tile's scores overflow to -inf, which leaves one half of the workgroup without weight; a row that sees no other tile is 0.
+    A query that is not a number beside them.  (Scores of -512: their maxima and sums are rounded by 2^-15, and half as much again
+    in the pass of the weights, which the exponential turns into 2^-13 of a weight.)"""
+    n, D = 600, 16
+    pages, plain = filled(ops, [n], 1, 1, D, weights=True)
+    q = torch.zeros((n, 2 * D), dtype=adt(act))
+    q[:, 0] = -2.0 ** 118
+    q[17, D + 4] = math.nan
+    lost = np.arange(plain.code["k"].shape[3]) // 64 % 2 == odd
+    plain.code["k"][0, 0, 0] = 0.0
+    plain.code["k"][0, 0, 0, :, 0] = np.where(lost, 1.0, 2.0 ** -9)
+    plain.scale["k"][0, 0, 0] = np.where(lost[::16], 2.0 ** 11, 2.0 ** -100)
+    P.fill_pages(pages, plain, D)
+    before = plain.weight[0, 0, 0].copy()
+    out = ops.attention_e4m3(q.to(DEV), pages, 0, 2, None, 1.0, act, make_runs([0], [0], [n]), add_weights=True).double().cpu().numpy().reshape(n, 2, D)
+    assert np.isnan(out[17, 1]).all() and np.isfinite(out[:17]).all() and np.isfinite(out[18:]).all() and np.isfinite(out[17, 0]).all()
+    keys, values = plain.values("k", 0, 0, 0)[:n], plain.values("v", 0, 0, 0)[:n]
+    seeing = np.arange(0 if odd else 64, n)
+    assert (out[:seeing[0], 0] == 0).all()
+    o, w, spread, _reach = P.attend(q.double().numpy()[seeing, :D], keys, values, seeing.tolist(), 1.0)
+    assert not w[lost[:n]].any()
+    rounding = 2.0 ** -8 if act == "bfloat16" else 0.0
+    assert (np.abs(out[seeing, 0] - o) <= ((rounding + 2.0 ** -13) * spread + rounding * np.abs(o)) * 1.01).all()
+    rest = np.concatenate([np.arange(17), np.arange(18, n)])
+    _o, w1, _s, _r = P.attend(np.zeros((n - 1, D)), keys, values, rest.tolist(), 1.0)
+    gave = P.read_pages(pages, D).weight[0, 0, 0]
+    assert np.isnan(gave[:18]).all() and (gave[n:] == before[n:]).all()
+    total = (before[:n] + w + w1)[18:]
+    assert (np.abs(gave[18:n] - total) <= (w + w1)[18:] * 2.0 ** -12 + total * 2.0 ** -22).all()
+
+
+# ------------------------------------------------------------------------------------------------ single tokens whose waves go through several runs
+def random_pages(ops, lens, G, D, seed=0):
+    """Pages of codes drawn at random (no NaN), with scales of 2^-6 to 2^-3."""
+    pages, g = make_pages(ops, len(lens), max(lens), 1, G, D, weights=True, seed=seed), torch.Generator().manual_seed(seed)
+    for t in (pages.k, pages.v):
+        code = torch.randint(0, 120, t.shape, generator=g, dtype=torch.uint8) + 128 * torch.randint(0, 2, t.shape, generator=g, dtype=torch.uint8)
+        t.view(torch.uint8).copy_(code)
+    for t in (pages.k_scale, pages.v_scale):
+        t.copy_(torch.exp2(torch.randint(-6, -2, t.shape, generator=g).float()))
+    pages.weight.copy_(torch.rand(pages.weight.shape, generator=g))
+    return pages
+
+
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("nh,G,D,lens,opts", [(16, 16, 32, [4500, 3999, 2100, 1300, 4097, 70, 3500, 4200], dict()),
+                                              (20, 20, 48, [4096, 3000, 1100, 4400, 3700, 2048], dict(window=3500)),
+                                              (32, 16, 80, [3900, 4000, 3100, 1025, 2500, 3333, 4100], dict(softcap=5.0))])
+def test_waves_that_go_through_several_runs(ops, act, nh, G, D, lens, opts):
+    """Outputs and weights have the bits of each sequence alone, whose waves take a run each, and are right."""
+    B = len(lens)
+    assert 64 * G * B > 6144       # more runs, of 64 at most to a sequence, than waves
+    pages = random_pages(ops, lens, G, D)
+    plain = P.read_pages(pages, D)
+    alone = ops.E4m3Pages(pages.k, pages.v, pages.k_scale, pages.v_scale, pages.table, pages.weight.clone())
+    q = (torch.randn((B, nh * D), generator=torch.Generator().manual_seed(3)) * 0.05).to(adt(act))
+    args = dict(softcap=opts.get("softcap"), add_weights=True)
+    got = ops.attention_e4m3(q.to(DEV), pages, 0, nh, opts.get("window"), 0.125, act, make_runs(list(range(B)), [n - 1 for n in lens], [1] * B), **args)
+    for b, n in enumerate(lens):
+        one = ops.attention_e4m3(q[b:b + 1].to(DEV), alone, 0, nh, opts.get("window"), 0.125, act, make_runs([b], [n - 1], [1]), **args)
+        assert torch.equal(one[0], got[b]), b
+    assert torch.equal(pages.weight, alone.weight)
+    after = P.read_pages(pages, D).weight
+    for b in (0, B - 1):
+        n, given, slack = lens[b], np.zeros((G, lens[b])), np.zeros((G, lens[b]))
+        for h in range(nh):
+            kvh = h // (nh // G)
+            o, w, spread, reach = P.attend(q[b].double().numpy().reshape(nh, D)[h][None], plain.values("k", b, 0, kvh)[:n], plain.values("v", b, 0, kvh)[:n],
+                                           [n - 1], 0.125, opts.get("window"), opts.get("softcap"))
+            e = (D + 16) * 2.0 ** -24 * reach + 2.0 ** -20 * reach * ("softcap" in opts) + opts.get("softcap", 0.0) * 2e-7 + 2.0 ** -21
+            rel = 2 * e + (2.0 ** -8 if act == "bfloat16" else 2.0 ** -22) + n * 2.0 ** -24
+            off = np.abs(got[b].double().cpu().numpy().reshape(nh, D)[h] - o[0])
+            assert (off <= rel * spread[0] * 1.01 + (np.abs(o[0]) * 2.0 ** -8 * 1.01 if act == "bfloat16" else 0.0)).all(), (b, h)
+            given[kvh] += w
+            slack[kvh] += w * (2 * e[0] + 2.0 ** -20)
+        total = plain.weight[b, 0, :, :n] + given
+        assert (np.abs(after[b, 0, :, :n] - total) <= slack + total * 2.0 ** -22 + 1e-12).all(), b
+
+
 # ------------------------------------------------------------------------------------------------ writes
 @pytest.mark.parametrize("act", ACTS)
 @pytest.mark.parametrize("rotary,pairing", [(256, 0), (256, 1), (254, 0), (254, 1)])
 def test_writes_at_the_most_shared_memory(ops, act, rotary, pairing):
     """The angles of 64 rows of heads of 256: 64 KiB, and what the kernel has beside them."""
     check_write(ops, act, 1, 1, 256, rotary, pairing, False, 64, [([0], [64]), ([0], [3]), ([0], [130])])
+
+
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("nh,G,D,rotary,pairing,bias,seqs,longest", [
+    (2, 16, 16, 16, 0, True, 12, 900), (3, 5, 48, 0, 0, False, 20, 900), (1, 5, 32, 20, 1, True, 60, 900), (1, 16, 32, 12, 0, False, 12, 900),
+    (1, 16, 144, 144, 0, True, 2, 2100)])
+def test_writes_of_several_kv_heads_to_a_workgroup(ops, act, nh, G, D, rotary, pairing, bias, seqs, longest):
+    """1,024 tiles times kv heads and more, most of which nothing falls into; first blocks that are there in part; rows of one head that
+    are not finite, which leave its workgroup's other heads as they are."""
+    assert ((longest + 62) // 64 + 1) * seqs * G >= 1024
+    rng = np.random.RandomState(seqs)
+    start, new = [(5 * i + 3) % 40 for i in range(seqs)], [1 + 7 * i % 40 for i in range(seqs)]
+    new[seqs // 3], new[seqs - 1] = longest, 130
+    slots, T = rng.permutation(seqs).tolist(), sum(new)
+    pages, plain = make_pages(ops, seqs, longest + 40, 1, G, D, weights=True), P.PlainPages(seqs, 1, G, D, -(-(longest + 40) // 64) * 64)
+    for s, n in zip(slots, start):
+        if n:
+            plain.write(s, 0, 0, rng.randn(n, G, D), rng.randn(n, G, D))
+    plain.weight[:] = 7.0
+    P.fill_pages(pages, plain, D)
+    W = (nh + 2 * G) * D
+    x, b = torch.randn((T, W), generator=torch.Generator().manual_seed(3)), (torch.randn((W,), generator=torch.Generator().manual_seed(4)) * 0.3).to(adt(act))
+    for t, head, number in ((7, nh + 3, math.nan), (150, nh + 3, math.inf), (150, nh + G + 1, 2.0 ** 121), (151, nh + G + 2, -math.inf), (T - 1, nh, math.nan)):
+        x[t, head * D + t % D] = number
+    positions = np.concatenate([np.arange(a, a + n) for a, n in zip(start, new)])
+    inv = (1e4 ** (-torch.arange(rotary // 2, dtype=torch.float64) / max(rotary // 2, 1))).float()
+    ops.rope_kv_write_e4m3(x.to(DEV), dev(positions.tolist()), inv.to(DEV), pairing, rotary, pages, 0, nh, act, make_runs(slots, start, new),
+                           bias=b.to(DEV) if bias else None)
+    full, t = (x + b.float() if bias else x).double().numpy().reshape(T, nh + 2 * G, D), 0
+    with np.errstate(invalid="ignore"):      # (infinities turn to NaN)
+        turned = P.rotate(full[:, nh:nh + G], positions, inv.double().numpy(), pairing)
+    for s, a, n in zip(slots, start, new):
+        plain.write(s, 0, a, turned[t:t + n], full[t:t + n, nh + G:])
+        t += n
+    got = P.read_pages(pages, D)
+    for m in "kv":
+        assert np.array_equal(got.scale[m], plain.scale[m])
+        assert_codes(got.code[m], plain.code[m]) if m == "k" and rotary else np.testing.assert_array_equal(got.code[m], plain.code[m])
+    assert np.array_equal(got.weight, plain.weight)
 
 
 @pytest.mark.parametrize("act", ACTS)
