@@ -47,6 +47,30 @@ def test_weights_of_a_prompt_with_a_query_that_is_not_a_number(ops, act, opts, r
     assert torch.equal(got.view(T, nh, D)[same.to(DEV)], want.view(T, nh, D)[same.to(DEV)])
 
 
+# ------------------------------------------------------------------------------------------------ capped scores
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("cap", [1.5, 30.0, 1000.0])
+@pytest.mark.parametrize("new", [1, 3])
+def test_weights_of_capped_scores(ops, act, cap, new):
+    """Scores that are eighths up to 1, without rounding.  In steps of 2^-24: the cap is off by 10 of a score (a quotient of sums of three, 2
+    for the reciprocal), which counts twice, by itself and in its row's sum; that sum by 32 (200 numbers, some by lanes, and the
+    exponential's 2); its logarithm, of 16 at most, and the difference from it by 8 each, rounded, and 16 more for the logarithm; the weight's own
+    exponential by 2: 86, of a weight, whatever the cap."""
+    n, D = 200, 16
+    pages, plain = filled(ops, [n], 1, 1, D, weights=True)
+    rng = np.random.RandomState(5)
+    plain.code["k"][0, 0, 0] = rng.randint(-8, 9, plain.code["k"][0, 0, 0].shape) / 8
+    plain.scale["k"][0, 0, 0], plain.weight[:] = 1.0, 0.0
+    P.fill_pages(pages, plain, D)
+    q = torch.zeros((new, 2 * D), dtype=adt(act))
+    q[:, 0], q[:, D + 3] = 1.0, -1.0
+    ops.attention_e4m3(q.to(DEV), pages, 0, 2, None, 1.0, act, make_runs([0], [n - new], [new]), softcap=cap, add_weights=True)
+    want = sum(P.attend(q[:, h * D:(h + 1) * D].double().numpy(), plain.values("k", 0, 0, 0)[:n], plain.values("v", 0, 0, 0)[:n],
+                        list(range(n - new, n)), 1.0, softcap=cap)[1] for h in range(2))
+    off = np.abs(P.read_pages(pages, D).weight[0, 0, 0, :n] - want) / want
+    assert off.max() <= 86 * 2.0 ** -24, off.max()
+
+
 # ------------------------------------------------------------------------------------------------ runs without tokens
 def padded(cu, slots, start, **kw):
     """Runs of a batch of single tokens, some of whose sequences bring none."""

@@ -29,6 +29,19 @@ typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 #define PIECES 1
 #endif
 
+// What becomes of a product (final_scores), worked out once on the host.
+struct Change {
+  float scale2, cap2;           // scale, cap in units of log2
+  float ky, k2;                 // scale / cap; 2 log2(e) scale / cap
+  float near[5];                // tanh(y) / y in powers of y^2, times scale2
+};
+static Change change_of(float scale, float cap) {
+  Change c{scale * LOG2E, cap * LOG2E, cap > 0.f ? scale / cap : 0.f, cap > 0.f ? 2.f * LOG2E * scale / cap : 0.f, {}};
+  const double p[5] = {0.99999998675739, -0.33333067944422656, 0.13324750504782334, -0.05298423882762508, 0.017131344428621548};
+  for (int i = 0; i < 5; ++i) c.near[i] = (float)(p[i] * (double)scale * 1.4426950408889634);
+  return c;
+}
+
 struct E4m3Attn {
   const act_t* q;               // [T][nh][hd]
   act_t* out;                   // [T][nh][hd]
@@ -38,6 +51,7 @@ struct E4m3Attn {
   int B, nh, nkv, window;
   float scale;
   ScoreMod mod;
+  Change ch;
   float* partial;               // decoding: [B][nh][max_runs][hd + 2]
   int max_runs;
   float* scores;                // with weights: decoding [B][nh][ld_scores], a column's scores in units of log2; prompts [B][cuts][nh][ld_scores], a
@@ -101,27 +115,52 @@ __device__ __forceinline__ float group_max(float v) { return with_lane_xor<32>(w
 __device__ __forceinline__ float group_sum(float v) { return with_lane_xor<32>(with_lane_xor<16>(v, LanesSum()), LanesSum()); }
 // Scores of a tile as the softmax takes them, and -inf where the column does not see the position, for one group of 16 columns.  MOD:
 // scaled, capped, biased, in units of log2; else (a positive scale alone) as the product left them, and the scale joins the exponent.
-// The cap in the bfloat16 library: cap tanh(x / cap) = cap - 2 cap / (e^(2 x / cap) + 1), which needs no bounds: e^.. may be 0 or infinite.
-struct Change {
-  float scale2, cap2, k2;      // scale, cap in units of log2; 2 log2(e) scale / cap
-};
-__device__ __forceinline__ Change change_of(const E4m3Attn& a) {
-  return Change{a.scale * LOG2E, a.mod.cap * LOG2E, a.mod.cap > 0.f ? 2.f * LOG2E * a.scale / a.mod.cap : 0.f};
+// The cap in the bfloat16 library, cap tanh(y) with y = x / cap, as good as 32 bits allow, for the weights that positions receive: up to |y| = 1/2
+// y P(y^2), P of degree 4 through tanh(y) / y at the five Chebyshev nodes (off by 1.3e-8 of itself); beyond, 1 - 2 / (e^(2 |y|) + 1), whose second term
+// is small enough there, and which needs no bounds: e^.. may be infinite.  (That one alone is off by 2^-23 of the cap, whatever the score:
+// 2e-6 of a weight at a cap of 50.)  A tile without large scores, as most are, passes the second form over.  In one that has some a score's own size
+// decides where weights come of it (`exact`: single tokens with weights, prompts' second pass); else the second form serves for all of the tile.
+// 2,048 tokens of 28 heads behind as many, a cap of 30, scores of a standard deviation of 0.9, 3.6 and 7.2: 167, 169 and 184 us, with weights 293, 297 and
+// 364 (175, 176 and 178, with weights 300, 298 and 300 with the second form alone).
+__device__ __forceinline__ float capped(float s, const Change& ch) {
+  const float y = s * ch.ky, z = y * y;
+  return s * fmaf(z, fmaf(z, fmaf(z, fmaf(z, ch.near[4], ch.near[3]), ch.near[2]), ch.near[1]), ch.near[0]);
+}
+__device__ __forceinline__ float capped_far(float s, const Change& ch) {
+  const float e = __builtin_amdgcn_exp2f(fabsf(s) * fabsf(ch.k2));
+  return copysignf(fmaf(-2.f * ch.cap2, __builtin_amdgcn_rcpf(e + 1.f), ch.cap2), s * ch.k2);
 }
 template <bool MOD>
-__device__ __forceinline__ void final_scores(f32x4 (&s)[4], const E4m3Attn& a, const Change& ch, float r1, float r2, int pos0, int p, int lo, bool masked) {
+__device__ __forceinline__ void final_scores(f32x4 (&s)[4], const E4m3Attn& a, bool exact, float r1, float r2, int pos0, int p, int lo, bool masked) {
   const int c = (threadIdx.x % 64) / 16;
   if constexpr (MOD) {
 #if defined(TQ_ACT_BF16)
     if (a.mod.cap > 0.f) {
+      float top = 0.f;
 #pragma unroll
       for (int jt = 0; jt < 4; ++jt)
 #pragma unroll
-        for (int v = 0; v < 4; ++v)
-          s[jt][v] = fmaf(-2.f * ch.cap2, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[jt][v] * ch.k2) + 1.f), ch.cap2);
+        for (int v = 0; v < 4; ++v) top = fmaxf(top, fabsf(s[jt][v]));
+      const bool far = __any(top * fabsf(a.ch.ky) > 0.5f);
+      if (far && exact) {
+#pragma unroll
+        for (int jt = 0; jt < 4; ++jt)
+#pragma unroll
+          for (int v = 0; v < 4; ++v) s[jt][v] = fabsf(s[jt][v] * a.ch.ky) > 0.5f ? capped_far(s[jt][v], a.ch) : capped(s[jt][v], a.ch);
+      } else if (far) {
+#pragma unroll
+        for (int jt = 0; jt < 4; ++jt)
+#pragma unroll
+          for (int v = 0; v < 4; ++v) s[jt][v] = capped_far(s[jt][v], a.ch);
+      } else {
+#pragma unroll
+        for (int jt = 0; jt < 4; ++jt)
+#pragma unroll
+          for (int v = 0; v < 4; ++v) s[jt][v] = capped(s[jt][v], a.ch);
+      }
     } else {
 #pragma unroll
-      for (int jt = 0; jt < 4; ++jt) s[jt] *= ch.scale2;
+      for (int jt = 0; jt < 4; ++jt) s[jt] *= a.ch.scale2;
     }
     if (a.mod.r1)
 #pragma unroll
@@ -219,7 +258,6 @@ struct DecodeWave {
   int kvh, p, lo, h, r, c;
   bool valid;
   float r1, r2;
-  Change ch;
   bf16x8 qf[2 * (DT / 4)][PIECES];
   u32x4 k[4][DT / 4], v[DT];
   f32x4 ks, vs;
@@ -237,7 +275,6 @@ struct DecodeWave {
     row = a.pages.table + (int64_t)a.slots[b] * a.pages.bt_stride;
     r1 = MOD && a.mod.r1 ? a.mod.r1[h] : 0.f;
     r2 = MOD && a.mod.r1 ? a.mod.r2[h] : 0.f;
-    ch = change_of(a);
     clear();
   }
   // (behind the first tile's codes, which are then on their way)
@@ -301,14 +338,14 @@ struct DecodeWave {
         }
     }
     if (next >= 0) fetch_k(next);
-    final_scores<MOD>(s, a, ch, r1, r2, pos0, p, lo, pos0 + E4M3_TILE - 1 > p || pos0 < lo);
+    final_scores<MOD>(s, a, a.scores != nullptr, r1, r2, pos0, p, lo, pos0 + E4M3_TILE - 1 > p || pos0 < lo);
     if (a.scores && valid) {
       float* at = a.scores + ((int64_t)b * a.nh + h) * a.ld_scores + pos0 + 4 * c;
 #pragma unroll
-      for (int jt = 0; jt < 4; ++jt) *reinterpret_cast<f32x4*>(at + 16 * jt) = MOD ? s[jt] : s[jt] * ch.scale2;
+      for (int jt = 0; jt < 4; ++jt) *reinterpret_cast<f32x4*>(at + 16 * jt) = MOD ? s[jt] : s[jt] * a.ch.scale2;
     }
     bf16x8 pf[2][PIECES];
-    softmax_tile<DT>(s, o, m, l, MOD ? 1.f : ch.scale2, pf);
+    softmax_tile<DT>(s, o, m, l, MOD ? 1.f : a.ch.scale2, pf);
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
@@ -566,7 +603,6 @@ __global__ __launch_bounds__(256 * HALVES) __attribute__((amdgpu_waves_per_eu(DT
   const int start = a.start[b], kvh = h / (a.nh / a.nkv);
   const int* row = a.pages.table + (int64_t)a.slots[b] * a.pages.bt_stride;
   const float r1 = MOD && a.mod.r1 ? a.mod.r1[h] : 0.f, r2 = MOD && a.mod.r1 ? a.mod.r2[h] : 0.f;
-  const Change ch = change_of(a);
   const int wg_last = start + min(qb + 64 * QG, n) - 1;
   const int tile_beg = reach_lo(start + qb, a.window, a.mod.chunk) / E4M3_TILE, tile_end = wg_last / E4M3_TILE + 1;
   const int wq0 = qb + wave * 16 * QG;
@@ -687,8 +723,8 @@ __global__ __launch_bounds__(256 * HALVES) __attribute__((amdgpu_waves_per_eu(DT
       bf16x8 pf[QG][2][PIECES];
 #pragma unroll
       for (int g = 0; g < QG; ++g) {
-        final_scores<MOD>(s[g], a, ch, r1, r2, pos0, p[g], lo[g], masked);
-        softmax_tile<DT>(s[g], o[g], m[g], l[g], MOD ? 1.f : ch.scale2, pf[g]);
+        final_scores<MOD>(s[g], a, false, r1, r2, pos0, p[g], lo[g], masked);
+        softmax_tile<DT>(s[g], o[g], m[g], l[g], MOD ? 1.f : a.ch.scale2, pf[g]);
       }
       ask_v(1);
       if constexpr (AHEAD) __builtin_amdgcn_sched_barrier(0);
@@ -775,7 +811,6 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DT * PIECES
   const int pos0 = tile * E4M3_TILE;
   const bool has = pos0 < start + n;
   const int* row = a.pages.table + (int64_t)a.slots[b] * a.pages.bt_stride;
-  const Change ch = change_of(a);
   const float r1 = MOD && a.mod.r1 ? a.mod.r1[h] : 0.f, r2 = MOD && a.mod.r1 ? a.mod.r2[h] : 0.f;
   bf16x8 kf[4][KS];
   {
@@ -853,11 +888,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DT * PIECES
       const float sum = lses[buf][16 * half + r];
       // every token of the 16 sees the whole tile: nothing to compare
       const bool masked = q1 + 15 >= n || start + q1 < pos0 + E4M3_TILE - 1 || reach_lo(start + q1 + 15, a.window, a.mod.chunk) > pos0;
-      final_scores<MOD>(s, a, ch, r1, r2, pos0, p, lo, false);
+      final_scores<MOD>(s, a, true, r1, r2, pos0, p, lo, false);
 #pragma unroll
       for (int jt = 0; jt < 4; ++jt)
 #pragma unroll
-        for (int v = 0; v < 4; ++v) s[jt][v] = __builtin_amdgcn_exp2f(fmaf(s[jt][v], MOD ? 1.f : ch.scale2, -sum));
+        for (int v = 0; v < 4; ++v) s[jt][v] = __builtin_amdgcn_exp2f(fmaf(s[jt][v], MOD ? 1.f : a.ch.scale2, -sum));
       // (by its place, not by a score of -inf: the sum of a row that is not a number is none either, and would reach positions it does not see)
       if (masked) {
         asm volatile("");      // (a branch, as in final_scores)
@@ -1005,7 +1040,7 @@ TQ_API int tq_e4m3_attention(const void* q, void* out, const int* cu, const int*
   if (!e4m3_pages_fit(page_size, heads, head0, nkv, hd) || nh % nkv != 0 || nh > 65535 || nh / nkv > 1024 || B > 65535) return TQ_ERR_UNSUPPORTED;
   if (!scratch && tq_e4m3_attention_scratch(T, B, nh, nkv, hd, max_new, max_end, decode, weight != nullptr)) return TQ_ERR_BAD_ARG;
   E4m3Attn a{(const act_t*)q, (act_t*)out, cu, slots, start, B, nh, nkv, window, scale, ScoreMod{softcap, r1, r2, chunk, sink, nullptr, 0},
-             nullptr, e4m3_most_runs(max_end, nh / nkv), nullptr, 0, nullptr,
+             change_of(scale, softcap), nullptr, e4m3_most_runs(max_end, nh / nkv), nullptr, 0, nullptr,
              E4m3Pages{(uint8_t*)k, (uint8_t*)v, (float*)k_scale, (float*)v_scale, weight, table, bt_stride, page_size, heads, head0, hd}};
   if (weight) {      // (first: its rows are read and written 16 bytes at a time)
     a.ld_scores = (max_end + E4M3_TILE - 1) / E4M3_TILE * E4M3_TILE;
