@@ -187,7 +187,7 @@ class Engine:
         """Lets positions of every sequence in ``slots`` go that holds more than ``keep``: every layer and kv head keeps the first
         ``first`` of them, the last ``recent`` (default: half of ``keep``), and of the others those that have received the most
         attention since they were written, ``keep`` in all.  Keys stay rotated as they were, and later tokens go on at the positions
-        that they would have had.  Needs pages for ``keep`` positions until each sequence is done (``CacheFull`` otherwise)."""
+        that they would have had, beyond those that the model was made for too.  Needs pages for ``keep`` positions until each sequence is done (``CacheFull`` otherwise)."""
         why = self.no_eviction()
         if why is not None:
             raise StepError(f"positions cannot be let go: {why}")
