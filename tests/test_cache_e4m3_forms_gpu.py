@@ -52,8 +52,8 @@ def test_weights_of_a_prompt_with_a_query_that_is_not_a_number(ops, act, opts, r
 @pytest.mark.parametrize("cap", [1.5, 30.0, 1000.0])
 @pytest.mark.parametrize("new", [1, 3])
 def test_weights_of_capped_scores(ops, act, cap, new):
-    """Scores that are eighths up to 1, without rounding.  In steps of 2^-24: the cap is off by 10 of a score (a quotient of sums of three, 2
-    for the reciprocal), which counts twice, by itself and in its row's sum; that sum by 32 (200 numbers, some by lanes, and the
+    """Scores that are eighths up to 1, without rounding.  In steps of 2^-24: the cap is off by 10 of a score (its argument, the argument's
+    square, five terms and their product with the score, a rounding or two each), which counts twice, by itself and in its row's sum; that sum by 32 (200 numbers, some by lanes, and the
     exponential's 2); its logarithm, of 16 at most, and the difference from it by 8 each, rounded, and 16 more for the logarithm; the weight's own
     exponential by 2: 86, of a weight, whatever the cap."""
     n, D = 200, 16
